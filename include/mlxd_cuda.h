@@ -132,6 +132,17 @@ int  mlxd_cuda_kv_gather(mlxd_kv *kv, int layer, int is_value, int pos, int n,
                          void *dst_dev, void *stream);
 int  mlxd_cuda_kv_set_offset(mlxd_kv *kv, int offset, void *stream);
 
+/* A cache of a given shape without a model, for callers that drive layers
+   themselves (no reference counterpart: the reference's cache grows with the
+   model's layers). window > 0 makes it a ring, as a windowed model's cache
+   is; the ring then keeps the rows of positions [0, sinks) for good: position
+   p lies in slot p below `sinks`, and in slot sinks + (p - sinks) %
+   (capacity - sinks) above (capacity >= sinks + window; sinks needs a window).
+   kv_write, kv_gather, kv_read and kv_attend follow this mapping; the model
+   calls (forward, step_async, generate) take only caches of kv_create. */
+int  mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int head_dim,
+                               int capacity, int window, int sinks);
+
 /* ---- forward (model_forward, emodel.c:221-337) --------------------------
    ids: n token ids (host or device memory). Appends n positions to kv.
    want_logits: write the last position's logits (bf16 [V]) to logits_dev
@@ -184,6 +195,89 @@ int  mlxd_cuda_linear_timed_chained(const mlxd_linear *const *ls, int n, int ite
 int  mlxd_cuda_rmsnorm(const void *x, int rows, int n, const void *w, float eps,
                        void *y, void *stream);
 
+/* Rotary positions (fwd_rope's mlx_fast_rope, forward.c:386-456, with the
+   interleaved pairing and the linear and YaRN scalings besides). */
+enum { MLXD_ROPE_DEFAULT = 0, MLXD_ROPE_LINEAR = 1, MLXD_ROPE_LLAMA3 = 2, MLXD_ROPE_YARN = 3 };
+typedef struct {
+    float theta;               /* base: pair i turns by p * theta^(-2i/dims), scaled */
+    int   dims;                /* rotated leading features of a head: even, 0 .. head_dim;
+                                  the rest is copied (0: all of it) */
+    int   interleaved;         /* pairs (2i, 2i + 1) instead of (i, i + dims/2) */
+    int   scaling;             /* MLXD_ROPE_* */
+    float factor;              /* linear, llama3, yarn: context extension, >= 1 */
+    float lo, hi;              /* llama3: low/high frequency factors; yarn: beta slow/fast */
+    int   orig_max;            /* llama3, yarn: positions of the original context */
+    float magnitude;           /* yarn: factor on cos and sin; 0: 0.1 ln(factor) + 1 */
+} mlxd_rope;
+/* y = x with the first `dims` features of every head rotated by their
+   position: n tokens x heads of head_dim (2 .. 256) features, bf16 or f32 (dtype),
+   token and head strides in elements for x and y. Token t is at position
+   pos_dev[t] (device int32), or pos + t when pos_dev is NULL. Angles are
+   reduced in f64 (exact to f32 at any int32 position), the rotation is in f32
+   and rounded once. y may be x itself with the same strides; any other
+   overlap is an error of the caller. n = 0 does nothing. */
+int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, int64_t x_token_stride,
+                    int64_t x_head_stride, const mlxd_rope *r, const int32_t *pos_dev, int pos, void *y,
+                    int64_t y_token_stride, int64_t y_head_stride, void *stream);
+
+/* Attention over the rows of one cache layer (the attention half of
+   fwd_attention, forward.c:495-795, on bf16 tensor cores with f32 softmax
+   statistics instead of the model path's fixed-association arithmetic):
+   n query tokens at positions pos .. pos + n - 1, out_i = softmax(scale *
+   q_i . k_j) v_j over the keys j <= pos + i that lie in the window
+   (pos + i - j < window; window 0: every key) or among the first `sinks`
+   positions. The rows of every visible position must have been written;
+   other rows may hold anything. q: bf16 [n][n_heads][head_dim] with
+   q_stride elements between tokens, out likewise; both 16-byte aligned, the
+   strides multiples of 8 elements and at least n_heads * head_dim. Query head
+   h reads kv head h / (n_heads / n_kv_heads). ws: a device workspace of
+   attn_workspace_bytes(), 256-byte aligned, that no other call in flight
+   uses (calls on one stream may share it). A wrapped ring takes at most
+   capacity - cache sinks - window + 1 queries a call, and no more sinks than
+   the cache keeps. Softmax weights are rounded to bf16 for the tensor cores
+   (values times unrounded statistics of the rounded weights); a non-finite
+   value row that one query sees may reach other queries of the same call. */
+typedef struct {
+    int   n_heads;             /* query heads, a multiple of the cache's kv heads */
+    int   window;              /* > 0: keys within the last `window` positions */
+    int   sinks;               /* with a window: first positions that stay visible */
+    float scale;               /* 0: 1 / sqrt(head_dim) */
+} mlxd_attn;
+size_t mlxd_cuda_attn_workspace_bytes(int head_dim);
+int  mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_stride, int n, int pos,
+                         const mlxd_attn *a, void *out, int64_t out_stride, void *ws, size_t ws_bytes,
+                         void *stream);
+
+/* A batch of sequences that share a prefix (n samples of one prompt; no
+   reference counterpart): positions [0, prefix_len) are rows of `prefix`
+   (unwrapped, unchanged and alive while the group is), each sequence's
+   further positions are rows of its own tail of up to tail_capacity tokens,
+   held by the group. */
+typedef struct mlxd_kv_group mlxd_kv_group;
+int  mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int prefix_len, int n_seqs,
+                               int tail_capacity);
+void mlxd_cuda_kv_group_destroy(mlxd_kv_group *g);
+/* Tail rows [row, row + n) of one sequence from contiguous device arrays
+   [Hkv][n][D] (kv_write's form). */
+int  mlxd_cuda_kv_group_write(mlxd_kv_group *g, int layer, int seq, int row, int n, const void *k_dev,
+                              const void *v_dev, void *stream);
+/* One decode step's new rows: tail row lens_dev[i] - 1 of every sequence i from
+   k and v (bf16 [n_seqs][Hkv][D], strides in elements between sequences,
+   multiples of 8, 16-byte aligned). A sequence whose length is outside
+   1 .. tail_capacity is skipped. */
+int  mlxd_cuda_kv_group_append(mlxd_kv_group *g, int layer, const void *k, int64_t k_stride, const void *v,
+                               int64_t v_stride, const int32_t *lens_dev, void *stream);
+/* Attention of one query token per sequence, at position prefix_len +
+   lens_dev[i] - 1, over the prefix (read once for all sequences) and the
+   first lens_dev[i] rows of its own tail; window, sinks and the layouts as in
+   kv_attend. Lengths are read on the device: 0 sees the prefix alone, a
+   negative one marks a finished sequence whose output row is left as it was,
+   one above tail_capacity counts as tail_capacity. A row that sees no key is
+   zero. */
+int  mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, int64_t q_stride,
+                               const int32_t *lens_dev, const mlxd_attn *a, void *out, int64_t out_stride,
+                               void *ws, size_t ws_bytes, void *stream);
+
 /* ---- sampler (sampler.h:11-50) ------------------------------------------ */
 typedef struct {
     float temperature;          /* < 0.01: greedy */
@@ -204,6 +298,22 @@ int mlxd_cuda_sample(const void *logits_dev, int dtype, int V, const mlxd_sampli
                      const int32_t *ctx_dev, int n_ctx, uint64_t step,
                      int32_t *tok_dev, float *logprob_dev, uint8_t *keep_dev,
                      void *stream);
+
+/* Scores of given tokens (the raw logprob of sampler_sample_lazy,
+   sampler.c:269-380, for any token of any row, with the distribution's
+   entropy and its most likely tokens): for each of `rows` rows of V logits
+   (bf16 or f32, row_stride elements apart) logprobs[r] = log softmax(row)
+   [targets[r]], entropy[r] in nats, and the n_top (0 .. 32, at most V)
+   largest logits' ids in descending order, ties to the lower id, with their
+   logprobs ([rows][n_top]). Statistics are f32 with the largest term kept
+   apart, so that peaked rows lose nothing. Any output may be NULL; targets
+   may be NULL when logprobs is. -inf logits have probability zero; a row
+   without any other is an empty distribution: logprobs -inf, entropy 0, top
+   ids in index order. A row with +inf or NaN gives NaN scores (its ids order
+   NaN last). A target outside the row gives NaN. */
+int mlxd_cuda_token_scores(const void *logits_dev, int dtype, int rows, int V, int64_t row_stride,
+                           const int32_t *targets_dev, int n_top, float *logprobs_dev, float *entropy_dev,
+                           int32_t *top_ids_dev, float *top_logprobs_dev, void *stream);
 
 /* The pipelined decode loop's pair (engine.c:470-560 over
    mlxbridge_async_eval_n + mlxbridge_item_int32, mlxbridge.c:88-124):

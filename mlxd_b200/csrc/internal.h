@@ -16,6 +16,9 @@ bool cuda_ok(cudaError_t e, const char *what);
 
 void *dev_alloc(size_t bytes);      // tracked cudaMalloc (nullptr + error on failure)
 void dev_free(void *p);
+// p is memory of the current device (device or managed); false + error naming
+// `what` otherwise (host memory, another device's, null)
+bool on_device(const void *p, const char *what);
 
 // A projection in device memory. Every quantized matrix keeps its MLX
 // arrays (w u32 [rows][cols/8], scales/biases [rows][cols/group] of sdtype);
@@ -122,6 +125,8 @@ struct mlxd_model {
 struct mlxd_kv {
     int layers, hkv, d, cap;
     int window;                 // ring buffer when > 0
+    int sinks;                  // ring: slots [0, sinks) keep positions [0, sinks)
+    int device;                 // the device the cache was created on
     int offset;                 // absolute positions written (host mirror)
     uint16_t *k = nullptr, *v = nullptr;   // [L][hkv][cap][d]
     int32_t *d_pos = nullptr;   // device copy of offset (position of the next token)
@@ -129,5 +134,13 @@ struct mlxd_kv {
     // decode attention's per-step block results and arrival counters
     float *att_part = nullptr;
     int *att_cnt = nullptr;
-    int att_nbmax = 0, att_rep = 0;
+    int att_nbmax = 0, att_rep = 0;   // att_rep 0: a cache of kv_create_shape
+};
+
+// n sequences over a shared prefix: tails [L][n][hkv][cap][d]
+struct mlxd_kv_group {
+    const mlxd_kv *prefix;
+    int prefix_len, n, cap;
+    int layers, hkv, d, device;
+    uint16_t *k = nullptr, *v = nullptr;
 };

@@ -8,6 +8,7 @@
 #include <atomic>
 #include <chrono>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -556,6 +557,10 @@ static int generic_forward(mlxd_model *m, mlxd_kv *kv, const int32_t *ids_dev, i
 }
 
 static int check_room(const mlxd_model *m, const mlxd_kv *kv, int n) {
+    if (!kv->att_rep || kv->layers != m->c.layers || kv->hkv != m->hkv || kv->d != m->c.head_dim) {
+        set_error(kv->att_rep ? "KV cache made for another model shape" : "KV cache of kv_create_shape: the model takes kv_create's");
+        return -1;
+    }
     if (kv->offset + n > m->rope_positions) {
         set_error("position %d beyond the %d positions of this model's RoPE table", kv->offset + n,
                   m->rope_positions);
@@ -891,7 +896,12 @@ int mlxd_cuda_kv_create(mlxd_kv **out, const mlxd_model *m, int capacity) {
     kv->d = m->c.head_dim;
     kv->cap = capacity;
     kv->window = m->c.window;
+    kv->sinks = 0;
     kv->offset = 0;
+    if (!cuda_ok(cudaGetDevice(&kv->device), "kv_create")) {
+        delete kv;
+        return -1;
+    }
     if (kv->window > 0 && capacity < kv->window) {
         set_error("ring capacity %d smaller than the window %d", capacity, kv->window);
         delete kv;
@@ -915,6 +925,44 @@ int mlxd_cuda_kv_create(mlxd_kv **out, const mlxd_model *m, int capacity) {
     }
     if (!cuda_ok(cudaMemset(kv->d_pos, 0, 4), "memset") ||
         !cuda_ok(cudaMemset(kv->att_cnt, 0, (size_t)kv->hkv * 4), "memset")) {
+        mlxd_cuda_kv_destroy(kv);
+        return -1;
+    }
+    *out = kv;
+    return 0;
+}
+
+int mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int head_dim, int capacity, int window,
+                              int sinks) {
+    if (!out || layers <= 0 || n_kv_heads <= 0 || head_dim <= 0 || head_dim > 256 || head_dim % 8 || capacity <= 0 ||
+        window < 0 || sinks < 0) {
+        set_error("kv_create_shape: bad arguments (head_dim: a multiple of 8 up to 256)");
+        return -1;
+    }
+    if (sinks && !window) {
+        set_error("kv_create_shape: sinks without a window");
+        return -1;
+    }
+    if (window && (int64_t)sinks + window > capacity) {
+        set_error("ring capacity %d smaller than %d sinks and the window %d", capacity, sinks, window);
+        return -1;
+    }
+    mlxd_kv *kv = new (std::nothrow) mlxd_kv();
+    if (!kv) {
+        set_error("kv_create_shape: out of host memory");
+        return -1;
+    }
+    kv->layers = layers;
+    kv->hkv = n_kv_heads;
+    kv->d = head_dim;
+    kv->cap = capacity;
+    kv->window = window;
+    kv->sinks = sinks;
+    kv->offset = 0;
+    const size_t bytes = (size_t)layers * n_kv_heads * capacity * head_dim * 2;
+    if (!cuda_ok(cudaGetDevice(&kv->device), "kv_create_shape") || !(kv->k = (uint16_t *)dev_alloc(bytes)) ||
+        !(kv->v = (uint16_t *)dev_alloc(bytes)) || !(kv->d_pos = (int32_t *)dev_alloc(4)) ||
+        !cuda_ok(cudaMemset(kv->d_pos, 0, 4), "memset")) {
         mlxd_cuda_kv_destroy(kv);
         return -1;
     }
@@ -952,17 +1000,24 @@ int mlxd_cuda_kv_reset(mlxd_kv *kv) {
 }
 
 // rows [pos, pos + n) of every kv head of one layer, ring-aware, as 2-D
-// copies: dev [hkv][n][D] <-> cache slots (pos + i) % cap
+// copies: dev [hkv][n][D] <-> cache slots (pos + i) % cap (a ring with sinks:
+// slot p below `sinks`, the other slots the ring of the positions above)
 static int kv_rows(mlxd_kv *kv, int layer, bool value, int pos, int n, uint16_t *dev, bool to_cache,
                    cudaStream_t st) {
     if (!kv || layer < 0 || layer >= kv->layers || pos < 0 || n < 0 || n > kv->cap || !dev) {
         set_error("kv rows: bad arguments");
         return -1;
     }
+    const int ring = kv->cap - kv->sinks;
+    if (pos >= kv->sinks && n > ring) {
+        set_error("kv rows: %d rows over a ring of %d slots", n, ring);
+        return -1;
+    }
     const size_t layer_elems = (size_t)kv->hkv * kv->cap * kv->d, row = (size_t)kv->d * 2;
     uint16_t *base = (value ? kv->v : kv->k) + (size_t)layer * layer_elems;
-    for (int part = 0, done = 0; done < n; part++) {
-        const int slot = (pos + done) % kv->cap;
+    for (int done = 0; done < n;) {
+        const int p = pos + done;
+        const int slot = p < kv->sinks ? p : kv->sinks + (p - kv->sinks) % ring;
         const int len = n - done < kv->cap - slot ? n - done : kv->cap - slot;
         uint16_t *c = base + (size_t)slot * kv->d;
         uint16_t *d = dev + (size_t)done * kv->d;
@@ -1039,7 +1094,9 @@ int mlxd_cuda_kv_read(mlxd_kv *kv, int layer, int is_value, uint16_t *host_out, 
     const uint16_t *base = (is_value ? kv->v : kv->k) + (size_t)layer * layer_elems;
     for (int h = 0; h < kv->hkv; h++)
         for (int i = 0; i < live; i++) {
-            int slot = (first + i) % kv->cap;
+            // the sinks, then the ring's positions
+            const int p = i < kv->sinks ? i : first + i;
+            const int slot = p < kv->sinks ? p : kv->sinks + (p - kv->sinks) % (kv->cap - kv->sinks);
             MLXD_CHECK(cudaMemcpy(host_out + ((size_t)h * live + i) * kv->d,
                                   base + ((size_t)h * kv->cap + slot) * kv->d, (size_t)kv->d * 2,
                                   cudaMemcpyDeviceToHost));

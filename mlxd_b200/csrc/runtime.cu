@@ -58,6 +58,25 @@ void dev_free(void *p) {
     cudaFree(p);
 }
 
+bool on_device(const void *p, const char *what) {
+    int dev = 0;
+    cudaPointerAttributes a;
+    if (!p) {
+        set_error("%s: null pointer", what);
+        return false;
+    }
+    if (!cuda_ok(cudaGetDevice(&dev), what) || !cuda_ok(cudaPointerGetAttributes(&a, p), what)) return false;
+    if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) {
+        set_error("%s: not device memory", what);
+        return false;
+    }
+    if (a.type == cudaMemoryTypeDevice && a.device != dev) {
+        set_error("%s: memory of device %d, the current device is %d", what, a.device, dev);
+        return false;
+    }
+    return true;
+}
+
 }  // namespace mlxd
 
 using namespace mlxd;

@@ -53,6 +53,30 @@ def sampling(temperature=1.0, top_p=1.0, top_k=-1, min_p=0.0, seed=-1,
                     repetition_context)
 
 
+ROPE_DEFAULT, ROPE_LINEAR, ROPE_LLAMA3, ROPE_YARN = 0, 1, 2, 3
+
+
+class RopeConfig(C.Structure):
+    """mlxd_rope: rotary base, layout and context scaling."""
+    _fields_ = [("theta", C.c_float), ("dims", C.c_int), ("interleaved", C.c_int),
+                ("scaling", C.c_int), ("factor", C.c_float), ("lo", C.c_float), ("hi", C.c_float),
+                ("orig_max", C.c_int), ("magnitude", C.c_float)]
+
+
+def rope_config(theta, dims, interleaved=False, scaling=ROPE_DEFAULT, factor=1.0, lo=1.0, hi=4.0,
+                orig_max=8192, magnitude=0.0):
+    return RopeConfig(theta, dims, int(interleaved), scaling, factor, lo, hi, orig_max, magnitude)
+
+
+class AttnConfig(C.Structure):
+    """mlxd_attn: query heads, window, sinks and scale of one attention call."""
+    _fields_ = [("n_heads", C.c_int), ("window", C.c_int), ("sinks", C.c_int), ("scale", C.c_float)]
+
+
+def attn_config(n_heads, window=0, sinks=0, scale=0.0):
+    return AttnConfig(n_heads, window, sinks, scale)
+
+
 PREFILL_HOOK = C.CFUNCTYPE(None, C.c_void_p, C.c_int, C.c_int)
 STEP_HOOK = C.CFUNCTYPE(None, C.c_void_p, C.c_int)
 SEED_HOOK = C.CFUNCTYPE(None, C.c_void_p)
@@ -130,6 +154,21 @@ _SIGS = {
     "mlxd_cuda_kv_write": (C.c_int, [P, C.c_int, C.c_int, C.c_int, P, P, P]),
     "mlxd_cuda_kv_gather": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, P, P]),
     "mlxd_cuda_kv_set_offset": (C.c_int, [P, C.c_int, P]),
+    "mlxd_cuda_kv_create_shape": (C.c_int, [C.POINTER(P), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
+                                            C.c_int]),
+    "mlxd_cuda_rope": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int64, C.c_int64,
+                                 C.POINTER(RopeConfig), P, C.c_int, P, C.c_int64, C.c_int64, P]),
+    "mlxd_cuda_attn_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "mlxd_cuda_kv_attend": (C.c_int, [P, C.c_int, P, C.c_int64, C.c_int, C.c_int,
+                                      C.POINTER(AttnConfig), P, C.c_int64, P, C.c_size_t, P]),
+    "mlxd_cuda_kv_group_create": (C.c_int, [C.POINTER(P), P, C.c_int, C.c_int, C.c_int]),
+    "mlxd_cuda_kv_group_destroy": (None, [P]),
+    "mlxd_cuda_kv_group_write": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, P, P, P]),
+    "mlxd_cuda_kv_group_append": (C.c_int, [P, C.c_int, P, C.c_int64, P, C.c_int64, P, P]),
+    "mlxd_cuda_kv_group_attend": (C.c_int, [P, C.c_int, P, C.c_int64, P, C.POINTER(AttnConfig), P,
+                                            C.c_int64, P, C.c_size_t, P]),
+    "mlxd_cuda_token_scores": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int64, P, C.c_int, P, P, P,
+                                         P, P]),
     "mlxd_cuda_synth_quantized": (C.c_int, [P, P, P, C.c_int, C.c_int, C.c_int, C.c_uint64,
                                             C.c_float, P]),
     "mlxd_cuda_synth_bf16": (C.c_int, [P, C.c_size_t, C.c_uint64, C.c_float, C.c_float, P]),
@@ -168,6 +207,11 @@ def check(rc, what=""):
 
 def ptr(a):
     return C.c_void_p(a.ctypes.data)
+
+
+def dev_ptr(a):
+    """Device address of a DeviceBuffer or of a tensor with data_ptr()."""
+    return a.ptr if isinstance(a, DeviceBuffer) else C.c_void_p(a.data_ptr())
 
 
 # ------------------------------------------------------------ device memory
@@ -421,6 +465,22 @@ class KVCache:
         check(lib().mlxd_cuda_kv_create(C.byref(kv), model.m, capacity), "kv_create")
         self.kv = kv
 
+    @classmethod
+    def shaped(cls, layers, n_kv_heads, head_dim, capacity, window=0, sinks=0):
+        """A cache of a given shape without a model (mlxd_cuda_kv_create_shape)."""
+        self = cls.__new__(cls)
+        self.model = None
+        kv = C.c_void_p()
+        check(lib().mlxd_cuda_kv_create_shape(C.byref(kv), layers, n_kv_heads, head_dim, capacity,
+                                              window, sinks), "kv_create_shape")
+        self.kv, self.shape = kv, (n_kv_heads, head_dim)
+        return self
+
+    def write(self, layer, pos, k, v, stream=None):
+        """kvcache_update: rows [pos, pos + n) from device arrays k, v [Hkv][n][D] (tensors)."""
+        check(lib().mlxd_cuda_kv_write(self.kv, layer, pos, k.shape[1], dev_ptr(k), dev_ptr(v), stream),
+              "kv_write")
+
     def offset(self, layer=0):
         return lib().mlxd_cuda_kv_offset(self.kv, layer)
 
@@ -431,14 +491,17 @@ class KVCache:
         check(lib().mlxd_cuda_kv_reset(self.kv), "kv_reset")
 
     def read(self, layer, value=False):
-        c = self.model.cfg
-        hkv = c.n_kv_heads // max(c.tp_size, 1)
+        if self.model is None:
+            hkv, head_dim = self.shape
+        else:
+            c = self.model.cfg
+            hkv, head_dim = c.n_kv_heads // max(c.tp_size, 1), c.head_dim
         cap = self.capacity(layer)
-        buf = np.zeros((hkv, cap, c.head_dim), dtype=np.uint16)
+        buf = np.zeros((hkv, cap, head_dim), dtype=np.uint16)
         n = C.c_int()
         check(lib().mlxd_cuda_kv_read(self.kv, layer, int(value), ptr(buf), C.byref(n)), "kv_read")
-        return np.ascontiguousarray(buf.reshape(-1)[: hkv * n.value * c.head_dim]).reshape(
-            hkv, n.value, c.head_dim)
+        return np.ascontiguousarray(buf.reshape(-1)[: hkv * n.value * head_dim]).reshape(
+            hkv, n.value, head_dim)
 
     def close(self):
         if getattr(self, "kv", None):
@@ -450,6 +513,37 @@ class KVCache:
             self.close()
         except Exception:
             pass
+
+
+class KVGroup:
+    """Sequences that share the first prefix_len positions of a cache, each with
+    its own tail (mlxd_kv_group)."""
+
+    def __init__(self, prefix, prefix_len, n_seqs, tail_capacity):
+        g = C.c_void_p()
+        check(lib().mlxd_cuda_kv_group_create(C.byref(g), prefix.kv, prefix_len, n_seqs, tail_capacity),
+              "kv_group_create")
+        self.g, self.prefix = g, prefix
+
+    def write(self, layer, seq, row, k, v, stream=None):
+        """Tail rows [row, row + n) of one sequence from device arrays k, v [Hkv][n][D] (tensors)."""
+        check(lib().mlxd_cuda_kv_group_write(self.g, layer, seq, row, k.shape[1], dev_ptr(k), dev_ptr(v),
+                                             stream), "kv_group_write")
+
+    def close(self):
+        if getattr(self, "g", None):
+            lib().mlxd_cuda_kv_group_destroy(self.g)
+            self.g = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def attn_workspace_bytes(head_dim):
+    return lib().mlxd_cuda_attn_workspace_bytes(head_dim)
 
 
 class Linear:
@@ -530,6 +624,39 @@ def sample(logits, sp, ctx=None, step=0):
     lp = float(dlp.to_array(np.float32, (1,))[0])
     keep = dkeep.to_array(np.uint8, (V,)).astype(bool)
     return tok, lp, keep
+
+
+def rope(x, cfg, pos):
+    """mlxd_cuda_rope on a host array [n][heads][D] (uint16 bf16 bits or f32): pos is the first
+    token's position or an array of n positions."""
+    x = np.ascontiguousarray(x)
+    n, heads, D = x.shape
+    dt = BF16 if x.dtype == np.uint16 else F32
+    if dt == F32:
+        x = x.astype(np.float32, copy=False)
+    dx, dy = DeviceBuffer.from_array(x), DeviceBuffer(x.nbytes)
+    per = None if np.isscalar(pos) else DeviceBuffer.from_array(np.asarray(pos, np.int32))
+    check(lib().mlxd_cuda_rope(dx.ptr, dt, n, heads, D, heads * D, D, C.byref(cfg),
+                               per.ptr if per else None, 0 if per else int(pos), dy.ptr, heads * D, D, None),
+          "rope")
+    return dy.to_array(x.dtype, x.shape)
+
+
+def token_scores(logits, targets, n_top=0):
+    """mlxd_cuda_token_scores on host rows [rows][V] (uint16 bf16 bits or f32): (logprobs, entropy,
+    top ids, top logprobs)."""
+    x = np.ascontiguousarray(logits)
+    rows, V = x.shape
+    dt = BF16 if x.dtype == np.uint16 else F32
+    if dt == F32:
+        x = x.astype(np.float32, copy=False)
+    dx, dt_ids = DeviceBuffer.from_array(x), DeviceBuffer.from_array(np.asarray(targets, np.int32))
+    lp, ent = DeviceBuffer(rows * 4), DeviceBuffer(rows * 4)
+    ids, tlp = DeviceBuffer(rows * n_top * 4), DeviceBuffer(rows * n_top * 4)
+    check(lib().mlxd_cuda_token_scores(dx.ptr, dt, rows, V, V, dt_ids.ptr, n_top, lp.ptr, ent.ptr, ids.ptr,
+                                       tlp.ptr, None), "token_scores")
+    return (lp.to_array(np.float32, rows), ent.to_array(np.float32, rows),
+            ids.to_array(np.int32, (rows, n_top)), tlp.to_array(np.float32, (rows, n_top)))
 
 
 # ----------------------------------------------------------- synthetic models
