@@ -602,7 +602,7 @@ static size_t da_smem(const AttnDecodeArgs &a) {
 
 // cudaFuncSetAttribute is per device: clusters above 8 CTAs allowed once per
 // (kernel, device)
-static bool nonportable_allowed(const void *kern) {
+bool nonportable_allowed(const void *kern) {
     static std::mutex mu;
     static std::vector<std::pair<const void *, int>> done;
     int dev = 0;

@@ -225,6 +225,28 @@ MLXD_DEV unsigned smid_() {
 MLXD_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 MLXD_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// ---- clusters: barrier over all CTAs, and loads of CTA `rank`'s shared memory
+MLXD_DEV void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+MLXD_DEV uint32_t cluster_addr(const void *p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+    return a;
+}
+MLXD_DEV float ld_cluster(const float *p, int rank) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(p, rank)));
+    return v;
+}
+MLXD_DEV float4 ld_cluster4(const float *p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(cluster_addr(p, rank)));
+    return v;
+}
+
 // D = A(16x16 bf16, row) * B(16x8 bf16, col) + C, f32 accumulate
 MLXD_DEV void mma_bf16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(

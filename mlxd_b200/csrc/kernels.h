@@ -10,6 +10,8 @@ int num_sms();
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per kernel, device
 // and size; false (error set) when the runtime refuses
 bool smem_allowed(const void *kern, size_t bytes);
+// clusters above 8 CTAs allowed for the kernel on this device (attention.cu)
+bool nonportable_allowed(const void *kern);
 
 // ---- projections (qgemv.cu). Every launcher computes the group-exact
 // arithmetic (gemv_i8.cuh): identical bits for decode, prefill and shards.

@@ -31,6 +31,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "tc.cuh"
 #include "gemv_i8.cuh"
 #include "kernels.h"
 
@@ -63,40 +64,10 @@ MLXD_DEV double int_times_pow2_hi(int v, int hi) {
     return __hiloint2double(hi, v ^ (int)0x80000000) - __hiloint2double(hi, (int)0x80000000);
 }
 
-// K-major operand with 128-byte rows in the 128B swizzle: 8-row atoms of
-// 1024 B (stride byte offset), leading offset unused (1), descriptor version 1
-MLXD_DEV uint64_t umma_desc_sw128(uint32_t saddr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-    d |= (uint64_t)1 << 16;                      // leading byte offset (16 B units)
-    d |= (uint64_t)(1024 >> 4) << 32;            // stride byte offset
-    d |= (uint64_t)1 << 46;                      // version
-    d |= (uint64_t)2 << 61;                      // SWIZZLE_128B
-    return d;
-}
 // kind::i8 instruction descriptor: s32 accumulator (2 at bit 4), A u8 (0 at
 // bit 7), B s8 (1 at bit 10), both K-major, N >> 3 at bit 17, M >> 4 at bit 24
 constexpr uint32_t umma_idesc_u8s8(int M, int N) {
     return (2u << 4) | (0u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
-}
-
-MLXD_DEV void mbar_arrive(uint64_t *bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-MLXD_DEV void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-MLXD_DEV void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-MLXD_DEV void tmem_ld16(uint32_t (&v)[16], uint32_t ta) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-        : "r"(ta));
-}
-MLXD_DEV void tmem_ld8(uint32_t (&v)[8], uint32_t ta) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
-                 : "r"(ta));
 }
 
 // 8 nibbles (elements 0..7, LSB first) of one MLX word widened to 8 bytes
@@ -410,11 +381,7 @@ __global__ void __launch_bounds__(XG_THREADS, 1)
 
 // ------------------------------------------------------------------ host
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                  const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn encode_fn() {
     static EncodeTiledFn fn = [] {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
