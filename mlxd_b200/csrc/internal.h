@@ -1,5 +1,6 @@
 // Internal structures of libmlxd_cuda (not part of the C ABI).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <stddef.h>
@@ -135,6 +136,8 @@ struct mlxd_kv {
     float *att_part = nullptr;
     int *att_cnt = nullptr;
     int att_nbmax = 0, att_rep = 0;   // att_rep 0: a cache of kv_create_shape
+    CUtensorMap map_k, map_v;   // all layers' rows for kv_attend's tiles
+    bool maps = false;
 };
 
 // n sequences over a shared prefix: tails [L][n][hkv][cap][d]

@@ -133,6 +133,9 @@ int attention_prefill(const uint16_t *q, int S, int pos0, const uint16_t *kc,
                       const uint16_t *gate_src, int qdim, uint16_t *out, float *scr, size_t scr_floats,
                       cudaStream_t st);
 
+// a new cache's tensor maps for the tile kernel (kv_attend.cu)
+void kv_attend_prepare(mlxd_kv *kv);
+
 // ---- sampler (sampler.cu)
 // The sampler's scratch for rows of up to V logits, owned by its caller (one
 // per model); d_nctx / d_step (optional): the context length and the draw's

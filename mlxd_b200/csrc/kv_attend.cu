@@ -6,10 +6,12 @@
 // over the keys j <= p_i with p_i - j < window or j < sinks, in one pass over
 // the keys with a running maximum m_i.
 #include <math.h>
+#include <mutex>
 #include <new>
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tc.cuh"
 
 namespace mlxd {
 
@@ -52,7 +54,7 @@ struct Span {
 };
 MLXD_DEV Span span_of(const AttnCall &c, int lo, int hi) {
     Span s;
-    s.a1 = min(c.sinks, lo);
+    s.a1 = min(min(c.sinks, lo), c.total);
     if (c.total <= c.cap) {
         s.b0 = lo;
         s.b1 = min(hi, c.total);
@@ -452,6 +454,444 @@ static int attend_few(const AttnCall &c, int rows, int keys, bool pdl, cudaStrea
     return -1;
 }
 
+// ---- many query rows per kv head: tensor-core tiles
+//
+// A CTA takes up to 256 query rows of one kv head (the head groups of
+// consecutive tokens, or of a batch's sequences: rows r = token * rep + head
+// in group, so that a key tile is read once for the whole group) and walks
+// the visible slots 128 at a time, in slot order: a ring needs no unwrapping.
+//
+//   warp 0, one lane   TMA: key tile j (128 slots x D, 128B swizzle) and value
+//                      tile j into their stages;
+//   warp 1, one lane   per query tile t (two of 128 rows) and key tile j:
+//                      S = Q K^T into TMEM, and once the softmax warps have
+//                      put the weights in place of S, O += P V (P from TMEM,
+//                      V as stored: its rows are the contraction);
+//   warps 4-7, 8-11    query tile 0 / 1, one row per thread: maximum and sum
+//                      of S over the key tile, P = e^(S - m) rounded to bf16
+//                      over S's own columns. O is rescaled only when a row's
+//                      maximum grew by more than 2^8 (the statistics are
+//                      relative to the maximum in use, so any will do).
+//
+// While one query tile is in its softmax the tensor cores work on the other.
+// The row sum adds the rounded weights, so that sum and numerator weigh alike.
+// Bound by the exponentials (128 x 128 per tile at 16 a clock and SM, 1024
+// clocks) and the tensor cores (2 x 512 clocks) alike when rows are many, by
+// HBM when a prefix is long and the rows are few.
+// Keys no row of the CTA sees may hold anything: their scores are masked and
+// their value rows zeroed in shared memory. Every wait is bounded; a launch
+// that gave up says so in a host word that the next call reports.
+constexpr int AT_THREADS = 384, AT_KT = 128, AT_ROWS = 256;
+
+template <int DB>
+struct AtLayout {
+    static constexpr int STAGES = DB == 1 ? 3 : 2;
+    static constexpr int BLOCK = AT_KT * 128;          // 128 rows x 64 features
+    static constexpr int TILE = DB * BLOCK;
+    static constexpr size_t Q = 0, K = 2 * TILE, V = K + STAGES * TILE, BARS = V + STAGES * TILE;
+    static constexpr size_t TOTAL = 1024 + BARS + 512;
+};
+
+struct TileCall {
+    int z0;                    // the layer's first kv head in the tensor maps
+    int splits;                // key splits (grid z)
+    float *part_o;             // partial results, or null: the whole result to out
+    float2 *part_ml;
+    int64_t prow;              // rows per split of the partial results
+    int *fail;
+};
+
+// bits x of a 32-slot word at s0 with lo <= s0 + x < hi
+MLXD_DEV uint32_t span_bits(int s0, int lo, int hi) {
+    const int l = min(max(lo - s0, 0), 32), h = min(max(hi - s0, 0), 32);
+    const uint32_t up = h == 32 ? 0xffffffffu : (1u << h) - 1u;
+    return l >= h ? 0u : up & (0xffffffffu << l);
+}
+MLXD_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <int DB>
+__global__ void __launch_bounds__(AT_THREADS, 1)
+    attend_tile_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                       const __grid_constant__ AttnCall c, const __grid_constant__ TileCall t) {
+    using L = AtLayout<DB>;
+    constexpr int NS = L::STAGES;
+    extern __shared__ __align__(1024) unsigned char at_raw[];
+    unsigned char *sm = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(sm + L::BARS);
+    uint64_t *kempty = kfull + NS, *vfull = kempty + NS, *vempty = vfull + NS;
+    uint64_t *sfull = vempty + NS, *pfull = sfull + 2, *odone = pfull + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(odone + 1);
+    __shared__ int s_pmin, s_pmax, s_fail;
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int head = blockIdx.y, rows = c.n * c.rep;
+    const int r0 = (gridDim.x - 1 - blockIdx.x) * AT_ROWS;   // the longest rows first
+    const int nq = rows - r0 > 128 ? 2 : 1;
+    if (tid == 0) {
+        for (int i = 0; i < NS; i++) {
+            mbar_init(&kfull[i], 1);
+            mbar_init(&kempty[i], 1);
+            mbar_init(&vfull[i], 1);
+            mbar_init(&vempty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&pfull[i], 4);
+        }
+        mbar_init(odone, 1);
+        s_pmin = INT32_MAX;
+        s_pmax = -1;
+        s_fail = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_trigger();   // every CTA is on an SM: the tails may start on free ones
+    // positions of the CTA's rows, and the query tiles (zero past the rows and D)
+    if (tid < AT_ROWS && r0 + tid < rows) {
+        const int p = query_pos(c, (r0 + tid) / c.rep);
+        if (p >= 0) {
+            atomicMin(&s_pmin, p);
+            atomicMax(&s_pmax, p);
+        }
+    }
+    for (int i = tid; i < nq * 128 * DB * 8; i += AT_THREADS) {
+        const int r = i / (DB * 8), ch = i % (DB * 8);   // 16-byte chunk of the row
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r0 + r < rows && ch * 8 < c.D) {
+            const int token = (r0 + r) / c.rep, qh = head * c.rep + (r0 + r) % c.rep;
+            v = ldg_nc_v4(c.q + token * c.q_stride + (int64_t)qh * c.D + ch * 8);
+        }
+        *reinterpret_cast<uint4 *>(sm + L::Q + (r >> 7) * L::TILE + (ch >> 3) * L::BLOCK + (r & 127) * 128 +
+                                   (((ch & 7) ^ (r & 7)) << 4)) = v;
+    }
+    fence_proxy_async();
+    __syncthreads();
+
+    // the visible slots as tiles: sinks, a ring's wrapped end, the rest
+    const int pmin = s_pmin, pmax = s_pmax;
+    int a1 = 0, c0 = 0, c1 = 0, b0 = 0, b1 = 0;      // tile ranges [0, a1), [c0, c1), [b0, b1)
+    Span all = {0, 0, 0, 0, 0};                      // the slots any row sees
+    if (pmax >= 0) {
+        all = span_of(c, window_lo(c, pmin), pmax + 1);
+        a1 = (all.a1 + AT_KT - 1) / AT_KT;
+        if (all.c1 > all.c0) {
+            c0 = max(all.c0 / AT_KT, a1);
+            c1 = max((all.c1 + AT_KT - 1) / AT_KT, c0);
+        }
+        if (all.b1 > all.b0) {
+            b0 = max(all.b0 / AT_KT, max(a1, c1));
+            b1 = max((all.b1 + AT_KT - 1) / AT_KT, b0);
+        }
+    }
+    const int nt = a1 + (c1 - c0) + (b1 - b0);
+    const int j0 = (int)((int64_t)nt * blockIdx.z / t.splits), j1 = (int)((int64_t)nt * (blockIdx.z + 1) / t.splits);
+    auto tile_slot = [&](int j) {
+        const int k = j < a1 ? j : j < a1 + c1 - c0 ? c0 + j - a1 : b0 + j - a1 - (c1 - c0);
+        return k * AT_KT;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint64_t mk = reinterpret_cast<uint64_t>(&tmk), mv = reinterpret_cast<uint64_t>(&tmv);
+            int kn = 0, vn = 0;                      // loads issued
+            bool ok = true;
+            auto load = [&](uint64_t map, uint64_t *full, uint64_t *empty, size_t base, int &n, int slot) {
+                const int st = n % NS, u = n / NS;
+                if (u > 0 && !mbar_wait(&empty[st], (u - 1) & 1)) return false;
+                mbar_expect_tx(&full[st], L::TILE);
+                n++;
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+                    asm volatile(
+                        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                        ::"r"(smem_u32(sm + base + st * L::TILE + b * L::BLOCK)), "l"(map), "r"(b * 64), "r"(slot),
+                        "r"(t.z0 + head), "r"(smem_u32(&full[st]))
+                        : "memory");
+                return true;
+            };
+            for (int j = j0; j < j1 && ok; j++) {
+                const int slot = tile_slot(j);
+                ok = load(mk, kfull, kempty, L::K, kn, slot) && load(mv, vfull, vempty, L::V, vn, slot);
+            }
+            if (!ok) s_fail = 1;
+            // after a failure: no copy may land once the CTA is gone
+            for (int i = 0; i < NS; i++) {
+                if (kn > i) mbar_wait(&kfull[(kn - 1 - i) % NS], ((kn - 1 - i) / NS) & 1);
+                if (vn > i) mbar_wait(&vfull[(vn - 1 - i) % NS], ((vn - 1 - i) / NS) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && j1 > j0) {
+            constexpr uint32_t iqk = umma_idesc_bf16(128, AT_KT, false), ipv = umma_idesc_bf16(128, DB * 64, true);
+            const uint32_t q0 = smem_u32(sm + L::Q), k0 = smem_u32(sm + L::K), v0 = smem_u32(sm + L::V);
+            auto qk = [&](int i, int n) {            // S_i = Q_i K_n^T
+                const uint32_t kt = k0 + (n % NS) * L::TILE, qt = q0 + i * L::TILE;
+#pragma unroll
+                for (int k = 0; k < DB * 4; k++) {
+                    const uint32_t off = (k >> 2) * L::BLOCK + (k & 3) * 32;
+                    asm volatile(
+                        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem + i * 128),
+                        "l"(umma_desc_sw128(qt + off)), "l"(umma_desc_sw128(kt + off)), "r"(iqk), "r"(k)
+                        : "memory");
+                }
+            };
+            auto pv = [&](int i, int n) {            // O_i += P_i V_n
+                const uint32_t vt = v0 + (n % NS) * L::TILE;
+#pragma unroll
+                for (int k = 0; k < AT_KT / 16; k++)
+                    asm volatile(
+                        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem + 256 + i * 128),
+                        "r"(tmem + i * 128 + k * 8), "l"(umma_desc_sw128_mn(vt + k * 2048, L::BLOCK)), "r"(ipv),
+                        "r"(n + k)
+                        : "memory");
+            };
+            const int nn = j1 - j0;
+            bool ok = mbar_wait(&kfull[0], 0);
+            if (ok) {
+                tc_fence_after();
+                for (int i = 0; i < nq; i++) {
+                    qk(i, 0);
+                    tc_commit(&sfull[i]);
+                }
+                tc_commit(&kempty[0]);
+            }
+            for (int n = 0; n < nn && ok; n++) {
+                for (int i = 0; i < nq && ok; i++) {
+                    if (i == 0) ok = mbar_wait(&vfull[n % NS], (n / NS) & 1);
+                    ok = ok && mbar_wait(&pfull[i], n & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    pv(i, n);
+                    if (n + 1 < nn) {
+                        if (i == 0) ok = mbar_wait(&kfull[(n + 1) % NS], ((n + 1) / NS) & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        qk(i, n + 1);
+                        tc_commit(&sfull[i]);
+                        if (i == nq - 1) tc_commit(&kempty[(n + 1) % NS]);
+                    }
+                    if (i == nq - 1) tc_commit(&vempty[n % NS]);
+                }
+            }
+            tc_commit(odone);
+            if (!mbar_wait(odone, 0) || !ok) s_fail = 1;
+        }
+    } else if (warp >= 4 && (warp - 4) / 4 < nq) {
+        const int wg = (warp - 4) >> 2, row = r0 + wg * 128 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
+        const float s2 = c.scale * LOG2E, slack = 8.0f / s2;
+        const int token = row / c.rep;
+        const int p = row < rows ? query_pos(c, token) : -1;
+        // what this row sees; rows that are not asked for see all (and are dropped)
+        Span sp = {0, 0, 0, 0, INT32_MAX};
+        if (p >= 0) sp = span_of(c, window_lo(c, p), p + 1);
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int n = 0; n < j1 - j0; n++) {
+            const int s0 = tile_slot(j0 + n);
+            uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
+            bool whole = s0 >= sp.b0 && s0 + AT_KT <= sp.b1;
+            if (!whole)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    see[w] = span_bits(s0 + 32 * w, 0, sp.a1) | span_bits(s0 + 32 * w, sp.c0, sp.c1) |
+                             span_bits(s0 + 32 * w, sp.b0, sp.b1);
+            whole = __all_sync(0xffffffffu, (see[0] & see[1] & see[2] & see[3]) == ~0u);
+            if (!__all_sync(0xffffffffu, mbar_wait(&sfull[wg], n & 1))) {
+                s_fail = 1;
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            uint32_t v[32];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                tmem_ld32(v, ts + 32 * w);
+                tmem_wait_ld();
+                if (whole) {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) mx = fmaxf(mx, __uint_as_float(v[x]));
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) mx = fmaxf(mx, see[w] >> x & 1 ? __uint_as_float(v[x]) : -INFINITY);
+                }
+            }
+            // a new maximum only when the old one is too far below
+            const bool grow = mx > m + slack || (m == -INFINITY && mx > -INFINITY);
+            if (__any_sync(0xffffffffu, grow)) {
+                const float a = grow ? ex2((m - mx) * s2) : 1.0f;
+                if (grow) m = mx;
+                l *= a;
+                if (n > 0)
+#pragma unroll
+                    for (int w = 0; w < DB * 2; w++) {
+                        tmem_ld32(v, to + 32 * w);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * a);
+                        tmem_st32(to + 32 * w, v);
+                    }
+            }
+            const float mu = m == -INFINITY ? 0.f : m * s2;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                tmem_ld32(v, ts + 32 * w);
+                tmem_wait_ld();
+                if (!whole)
+#pragma unroll
+                    for (int x = 0; x < 32; x++) v[x] = see[w] >> x & 1 ? v[x] : 0xff800000u;
+                uint32_t pk[16];
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    pk[x] = pack_bf2(ex2(fmaf(__uint_as_float(v[2 * x]), s2, -mu)),
+                                     ex2(fmaf(__uint_as_float(v[2 * x + 1]), s2, -mu)));
+                    l += lo_bf(pk[x]) + hi_bf(pk[x]);
+                }
+                tmem_st16(ts + 16 * w, pk);
+            }
+            tmem_wait_st();
+            // value rows of slots that no row sees: whatever they hold must not meet a zero weight
+            if (wg == 0 && !(s0 >= all.b0 && s0 + AT_KT <= all.b1)) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&vfull[n % NS], (n / NS) & 1))) {
+                    s_fail = 1;
+                    ok = false;
+                    break;
+                }
+                const int x = (warp & 3) * 32 + lane, s = s0 + x;
+                if (!(s < all.a1 || (s >= all.c0 && s < all.c1) || (s >= all.b0 && s < all.b1)))
+#pragma unroll
+                    for (int b = 0; b < DB; b++)
+#pragma unroll
+                        for (int q = 0; q < 8; q++)
+                            *reinterpret_cast<uint4 *>(sm + L::V + (n % NS) * L::TILE + b * L::BLOCK + x * 128 + q * 16) =
+                                make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[wg]);
+        }
+        const bool have = j1 > j0;
+        if (ok && have && !__all_sync(0xffffffffu, mbar_wait(odone, 0))) {
+            s_fail = 1;
+            ok = false;
+        }
+        tc_fence_after();
+        if (ok) {
+            const int64_t prow = (int64_t)token * c.hq + head * c.rep + row % c.rep;
+            const bool live = p >= 0;
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? l : 0.f);
+#pragma unroll
+            for (int w = 0; w < DB * 2; w++) {
+                uint32_t v[32];
+                __syncwarp();
+                if (have) {
+                    tmem_ld32(v, to + 32 * w);
+                    tmem_wait_ld();
+                }
+                if (live && have && t.part_o) {
+                    float *dst = t.part_o + (blockIdx.z * t.prow + prow) * c.D + 32 * w;
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4)
+                        if (32 * w + x < c.D)
+                            *reinterpret_cast<uint4 *>(dst + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                } else if (live && have) {
+                    uint16_t *dst = c.out + token * c.out_stride + (int64_t)(head * c.rep + row % c.rep) * c.D + 32 * w;
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8)
+                        if (32 * w + x < c.D) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                o[i] = pack_bf2(__uint_as_float(v[x + 2 * i]) * inv, __uint_as_float(v[x + 2 * i + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(dst + x) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+    if (tid == 0 && s_fail && t.fail) *reinterpret_cast<volatile int *>(t.fail) = 1;
+}
+
+// splits of every query row into its output row: one warp per row
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ AttnCall c) {
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), prow = (int64_t)c.n * c.hq;
+    if (row >= prow) return;
+    const float s2 = c.scale * LOG2E;
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < c.parts; k++) M = fmaxf(M, c.part_ml[k * prow + row].x);
+    const int d = lane * 4;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < c.parts; k++) {
+        const float2 ml = c.part_ml[k * prow + row];
+        if (ml.x == -INFINITY) continue;
+        const float a = ex2((ml.x - M) * s2);
+        L = fmaf(a, ml.y, L);
+        if (d < c.D) {
+            const float4 v = *reinterpret_cast<const float4 *>(c.part_o + (k * prow + row) * c.D + d);
+            acc.x = fmaf(a, v.x, acc.x);
+            acc.y = fmaf(a, v.y, acc.y);
+            acc.z = fmaf(a, v.z, acc.z);
+            acc.w = fmaf(a, v.w, acc.w);
+        }
+    }
+    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    if (d < c.D)
+        *reinterpret_cast<uint2 *>(c.out + row / c.hq * c.out_stride + row % c.hq * c.D + d) =
+            make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+}
+
+// the partial results' room in a workspace: 148 CTAs of 256 rows, whatever
+// the call (more rows than that go unsplit, or in batches)
+constexpr int64_t AT_WS_ROWS = 148 * AT_ROWS;
+static size_t at_ws_bytes(int D) { return (size_t)AT_WS_ROWS * ((D + 7) / 8 * 8 * 4 + 8) + 256; }
+
+template <int DB>
+static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &mk, const CUtensorMap &mv,
+                       cudaStream_t st) {
+    auto kern = attend_tile_kernel<DB>;
+    if (!smem_allowed((const void *)kern, AtLayout<DB>::TOTAL)) return -1;
+    const int64_t pairs = ((int64_t)c.n * c.rep + AT_ROWS - 1) / AT_ROWS;
+    kern<<<dim3((unsigned)pairs, c.hkv, t.splits), AT_THREADS, AtLayout<DB>::TOTAL, st>>>(mk, mv, c, t);
+    MLXD_CHECK(cudaGetLastError());
+    return 0;
+}
+
+// key splits of a tile launch: one wave of CTAs when the query tiles alone
+// would leave SMs idle, never more than the key tiles or the workspace's rows
+static int tile_splits(const AttnCall &c, int keys) {
+    const int64_t pairs = ((int64_t)c.n * c.rep + AT_ROWS - 1) / AT_ROWS * c.hkv, rows = (int64_t)c.n * c.hq;
+    int64_t s = num_sms() / pairs;
+    if (s > (keys + AT_KT - 1) / AT_KT) s = (keys + AT_KT - 1) / AT_KT;
+    if (s > AT_WS_ROWS / rows) s = AT_WS_ROWS / rows;
+    return s < 1 ? 1 : (int)s;
+}
+
 // tail rows of one decode step: sequence blockIdx.x
 __global__ void group_append_kernel(const uint16_t *__restrict__ k, int64_t ks, const uint16_t *__restrict__ v,
                                     int64_t vs, const int32_t *__restrict__ lens, uint16_t *tk, uint16_t *tv, int hkv,
@@ -466,19 +906,125 @@ __global__ void group_append_kernel(const uint16_t *__restrict__ k, int64_t ks, 
     }
 }
 
-static int attend(const AttnCall &c, void *ws, size_t ws_bytes, cudaStream_t st) {
+// a word in host memory that a launch sets when it gave up on a wait; made
+// with the first cache (null before), read at every call
+static int *fail_word(bool make) {
+    static std::mutex mu;
+    static int *word = nullptr;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!word && make) {
+        if (cudaHostAlloc((void **)&word, 64, cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            cudaGetLastError();
+            word = nullptr;
+        } else {
+            *word = 0;
+        }
+    }
+    return word;
+}
+static bool gave_up(const char *what) {
+    volatile int *w = fail_word(false);
+    if (!w || !*w) return false;
+    *w = 0;
+    set_error("%s: an earlier attention launch gave up waiting on its pipeline", what);
+    return true;
+}
+
+// 128 slots x 64 features of [layers * heads][cap][D] bf16 rows, 128B swizzle,
+// zero past D and cap
+static bool row_map(CUtensorMap *m, const uint16_t *base, int heads, int cap, int D) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)cap, (cuuint64_t)heads};
+    cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)cap * D * 2};
+    cuuint32_t box[3] = {64, AT_KT, 1}, estr[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<uint16_t *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+void kv_attend_prepare(mlxd_kv *kv) {
+    fail_word(true);
+    kv->maps = kv->d % 8 == 0 && kv->d <= 128 && row_map(&kv->map_k, kv->k, kv->layers * kv->hkv, kv->cap, kv->d) &&
+               row_map(&kv->map_v, kv->v, kv->layers * kv->hkv, kv->cap, kv->d);
+}
+
+static int attend_tiles(AttnCall c, const mlxd_kv *kv, int layer, int splits, bool partial, void *ws, cudaStream_t st) {
+    if (!kv->maps) {
+        set_error("attention: the cache has no tensor maps (driver without cuTensorMapEncodeTiled)");
+        return -1;
+    }
+    TileCall t = {};
+    t.z0 = layer * kv->hkv;
+    t.splits = splits;
+    t.prow = (int64_t)c.n * c.hq;
+    if (partial) {
+        t.part_o = (float *)ws;
+        t.part_ml = (float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+    }
+    t.fail = fail_word(false);
+    return c.D <= 64 ? launch_tile<1>(c, t, kv->map_k, kv->map_v, st) : launch_tile<2>(c, t, kv->map_k, kv->map_v, st);
+}
+
+static int attend_rows(const AttnCall &c, cudaStream_t st) {
     const int64_t rows = (int64_t)c.n * c.hq;
     if ((rows + 3) / 4 > INT32_MAX) {
         set_error("attention: too many query rows");
         return -1;
     }
-    if (c.D <= 128 && !c.lens && (c.n == 1 || c.n * c.rep <= 16)) {
-        const int last = c.pos0 + c.n;
-        const int keys = c.window && (int64_t)c.window + c.n - 1 + c.sinks < last ? c.window + c.n - 1 + c.sinks : last;
-        return attend_few(c, c.n * c.rep, keys, false, st);
-    }
     attend_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(c);
     MLXD_CHECK(cudaGetLastError());
+    return 0;
+}
+
+static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
+    if (c.D > 128) return attend_rows(c, st);
+    const int64_t span = (int64_t)c.window + c.n - 1 + c.sinks;
+    const int keys = c.window && span < c.total ? (int)span : c.total;   // the most that one row group sees
+    if ((int64_t)c.n * c.rep <= 16 || c.n == 1) return attend_few(c, c.n * c.rep, keys, false, st);
+    if ((int64_t)c.n * c.rep > INT32_MAX - AT_ROWS || c.hkv > 65535) {
+        set_error("kv_attend: too many query rows");
+        return -1;
+    }
+    const int splits = tile_splits(c, keys);
+    if (attend_tiles(c, kv, layer, splits, splits > 1, ws, st)) return -1;
+    if (splits == 1) return 0;
+    c.part_o = (const float *)ws;
+    c.part_ml = (const float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+    c.parts = splits;
+    attend_join_kernel<<<(unsigned)(((int64_t)c.n * c.hq + 7) / 8), 256, 0, st>>>(c);
+    MLXD_CHECK(cudaGetLastError());
+    return 0;
+}
+
+// sequences in batches whose partial rows fit the workspace: the prefix on
+// tiles, then every sequence's tail, which joins the prefix's results
+static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
+    if (c.D > 128) return attend_rows(c, st);
+    const int64_t tail = (int64_t)c.hkv * c.tcap * c.D;
+    int64_t most = AT_WS_ROWS / c.hq < 65535 ? AT_WS_ROWS / c.hq : 65535;
+    if (most < 1) {
+        set_error("kv_group_attend: %d query heads", c.hq);
+        return -1;
+    }
+    const int n = c.n;
+    for (int64_t i = 0; i < n; i += most) {
+        AttnCall b = c;
+        b.n = (int)(n - i < most ? n - i : most);
+        b.q += i * c.q_stride;
+        b.out += i * c.out_stride;
+        b.lens += i;
+        b.tk += i * tail;
+        b.tv += i * tail;
+        if (c.prefix > 0) {
+            const int splits = tile_splits(b, c.prefix);
+            if (attend_tiles(b, kv, layer, splits, true, ws, st)) return -1;
+            b.part_o = (const float *)ws;
+            b.part_ml = (const float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+            b.parts = splits;
+        }
+        if (attend_few(b, b.rep, c.tcap, c.prefix > 0, st)) return -1;
+    }
     return 0;
 }
 
@@ -486,7 +1032,7 @@ static int attend(const AttnCall &c, void *ws, size_t ws_bytes, cudaStream_t st)
 static int attn_call(AttnCall &c, const char *what, int hkv, int D, const void *q, int64_t q_stride, int n,
                      const mlxd_attn *a, void *out, int64_t out_stride, const void *ws, size_t ws_bytes) {
     if (!a || a->n_heads <= 0 || a->n_heads % hkv || a->window < 0 || a->sinks < 0 || !(a->scale >= 0.f) ||
-        !isfinite(a->scale)) {
+        !isfinite(a->scale) || (a->scale > 0.f && a->scale < 1e-30f)) {
         set_error("%s: bad attention parameters (heads a multiple of %d, window and sinks not negative, scale finite)",
                   what, hkv);
         return -1;
@@ -536,8 +1082,7 @@ using namespace mlxd;
 extern "C" {
 
 size_t mlxd_cuda_attn_workspace_bytes(int head_dim) {
-    if (head_dim <= 0) return 0;
-    return 256;
+    return head_dim > 0 ? at_ws_bytes(head_dim) : 0;
 }
 
 int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_stride, int n, int pos,
@@ -566,7 +1111,7 @@ int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_s
             return -1;
         }
     }
-    if (!same_device(kv->device, "kv_attend")) return -1;
+    if (!same_device(kv->device, "kv_attend") || gave_up("kv_attend")) return -1;
     const size_t layer_elems = (size_t)kv->hkv * kv->cap * kv->d;
     c.k = kv->k + layer * layer_elems;
     c.v = kv->v + layer * layer_elems;
@@ -574,7 +1119,7 @@ int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_s
     c.ring_sinks = kv->sinks;
     c.pos0 = pos;
     c.total = total;
-    return attend(c, ws, ws_bytes, (cudaStream_t)stream);
+    return attend_cache(c, kv, layer, ws, (cudaStream_t)stream);
 }
 
 int mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int prefix_len, int n_seqs,
@@ -665,7 +1210,8 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     }
     AttnCall c = {};
     if (attn_call(c, "kv_group_attend", g->hkv, g->d, q, q_stride, g->n, a, out, out_stride, ws, ws_bytes) ||
-        !on_device(lens_dev, "kv_group_attend: lengths") || !same_device(g->device, "kv_group_attend"))
+        !on_device(lens_dev, "kv_group_attend: lengths") || !same_device(g->device, "kv_group_attend") ||
+        gave_up("kv_group_attend"))
         return -1;
     const size_t layer_elems = (size_t)g->hkv * g->prefix->cap * g->d;
     const size_t o = (size_t)layer * g->n * g->hkv * g->cap * g->d;
@@ -677,7 +1223,7 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     c.tv = g->v + o;
     c.tcap = g->cap;
     c.prefix = c.total = g->prefix_len;
-    return attend(c, ws, ws_bytes, (cudaStream_t)stream);
+    return attend_group(c, g->prefix, layer, ws, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -928,6 +928,7 @@ int mlxd_cuda_kv_create(mlxd_kv **out, const mlxd_model *m, int capacity) {
         mlxd_cuda_kv_destroy(kv);
         return -1;
     }
+    kv_attend_prepare(kv);
     *out = kv;
     return 0;
 }
@@ -966,6 +967,7 @@ int mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int hea
         mlxd_cuda_kv_destroy(kv);
         return -1;
     }
+    kv_attend_prepare(kv);
     *out = kv;
     return 0;
 }
