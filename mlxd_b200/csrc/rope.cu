@@ -27,6 +27,8 @@ struct RopeCall {
     const int32_t *pos;        // or null: pos0 + t
     int pos0, n, heads, dims, D;
     int tokens, hblock;        // tokens and heads per CTA
+    int per;                   // items of a head
+    unsigned per_mul, h_mul;   // ceil(2^32 / per), ceil(2^32 / hblock) (0: divisor 1)
     float mag;
     double turns[RP_MAXPAIRS]; // turns per position
 };
@@ -44,35 +46,79 @@ MLXD_DEV uint16_t rp_put<uint16_t>(float v) { return f2bf(v); }
 template <>
 MLXD_DEV float rp_put<float>(float v) { return v; }
 
-template <typename T, bool INTER>
-__global__ void __launch_bounds__(RP_THREADS) rope_kernel(const __grid_constant__ RopeCall c) {
-    __shared__ float2 cs[RP_MAXTOK][RP_MAXPAIRS];
-    const int pairs = c.dims / 2;
+// N elements of a row: one 16-byte access, or one element
+template <typename T, int N>
+struct alignas(N * sizeof(T)) RopeVec {
+    T e[N];
+};
+
+// An item is N pairs of one head (or N copied features): N = 8 (bf16) or 4 (f32)
+// when every row starts on 16 bytes and the pairs and the copied rest come in
+// whole vectors, else 1. Items run over (token, head, vector) with the
+// vector fastest, so that a warp's accesses are contiguous.
+template <typename T, bool INTER, int N>
+__global__ void __launch_bounds__(RP_THREADS, 8) rope_kernel(const __grid_constant__ RopeCall c) {
+    __shared__ __align__(16) float2 cs[RP_MAXTOK][RP_MAXPAIRS];
+    using V = RopeVec<T, N>;
+    const int pairs = c.dims / 2, nrot = pairs / N;
     const int t0 = blockIdx.x * c.tokens, nt = min(c.tokens, c.n - t0);
+    const int h0 = blockIdx.y * c.hblock, nh = min(c.hblock, c.heads - h0);
+    const int items = nt * nh * c.per;
+    struct At {
+        const T *x;
+        T *y;
+        int j, t;
+    };
+    auto at = [&](int i) {
+        const int th = __umulhi(i, c.per_mul) + (c.per_mul ? 0 : i), t = nt == 1 ? 0 : __umulhi(th, c.h_mul) + (c.h_mul ? 0 : th);
+        const int h = h0 + th - t * nh;
+        return At{(const T *)c.x + (t0 + t) * c.xt + h * c.xh, (T *)c.y + (t0 + t) * c.yt + h * c.yh, i - th * c.per, t};
+    };
+    // feature of the first and second vector of item j
+    auto first = [&](int j) { return j < nrot ? (INTER ? 2 * N * j : N * j) : c.dims + N * (j - nrot); };
+    const int second = INTER ? N : pairs;
     for (int i = threadIdx.x; i < nt * pairs; i += RP_THREADS) {
-        const int t = i / pairs, j = i % pairs;
+        const int t = nt == 1 ? 0 : i / pairs, j = i - t * pairs;
         const int p = c.pos ? c.pos[t0 + t] : c.pos0 + t0 + t;
-        const double a = (double)p * c.turns[j];
+        const double g = (double)p * c.turns[j];
         float si, co;
-        sincospif((float)(2.0 * (a - rint(a))), &si, &co);
-        cs[t][j] = make_float2(co * c.mag, si * c.mag);
+        sincospif((float)(2.0 * (g - rint(g))), &si, &co);
+        // element e of vector v at e * nrot + v: a warp's reads meet no bank twice
+        cs[t][j % N * nrot + j / N] = make_float2(co * c.mag, si * c.mag);
     }
     __syncthreads();
-    const int h0 = blockIdx.y * c.hblock, nh = min(c.hblock, c.heads - h0);
-    const int per = pairs + (c.D - c.dims);   // rotated pairs and copied features of a head
-    for (int i = threadIdx.x; i < nt * nh * per; i += RP_THREADS) {
-        const int j = i % per, th = i / per, t = th / nh, h = h0 + th % nh;
-        const T *x = (const T *)c.x + (t0 + t) * c.xt + h * c.xh;
-        T *y = (T *)c.y + (t0 + t) * c.yt + h * c.yh;
-        if (j < pairs) {
-            const int ia = INTER ? 2 * j : j, ib = INTER ? 2 * j + 1 : j + pairs;
-            const float a = rp_get<T>(x[ia]), b = rp_get<T>(x[ib]);
-            const float2 r = cs[t][j];
-            y[ia] = rp_put<T>(a * r.x - b * r.y);
-            y[ib] = rp_put<T>(a * r.y + b * r.x);
-        } else {
-            y[c.dims + j - pairs] = x[c.dims + j - pairs];
+    for (int i = threadIdx.x; i < items; i += RP_THREADS) {
+        const At p = at(i);
+        const int f = first(p.j);
+        const V a = *reinterpret_cast<const V *>(p.x + f);
+        if (p.j >= nrot) {
+            *reinterpret_cast<V *>(p.y + f) = a;
+            continue;
         }
+        const V b = *reinterpret_cast<const V *>(p.x + f + second);
+        T in[2 * N], out[2 * N];                     // pair e: in[ia(e)], in[ib(e)]
+        auto ia = [](int e) { return INTER ? 2 * e : e; };
+        auto ib = [](int e) { return INTER ? 2 * e + 1 : N + e; };
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            in[e] = a.e[e];
+            in[N + e] = b.e[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float2 r = cs[p.t][e * nrot + p.j];
+            const float u = rp_get<T>(in[ia(e)]), v = rp_get<T>(in[ib(e)]);
+            out[ia(e)] = rp_put<T>(u * r.x - v * r.y);
+            out[ib(e)] = rp_put<T>(u * r.y + v * r.x);
+        }
+        V ra, rb;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            ra.e[e] = out[e];
+            rb.e[e] = out[N + e];
+        }
+        *reinterpret_cast<V *>(p.y + f) = ra;
+        *reinterpret_cast<V *>(p.y + f + second) = rb;
     }
 }
 
@@ -114,11 +160,32 @@ static int rope_turns(const mlxd_rope &r, RopeCall &c) {
     return 0;
 }
 
-template <typename T>
-static int rope_launch(const RopeCall &c, bool inter, cudaStream_t st) {
-    dim3 grid((c.n + c.tokens - 1) / c.tokens, (c.heads + c.hblock - 1) / c.hblock);
-    if (inter) rope_kernel<T, true><<<grid, RP_THREADS, 0, st>>>(c);
-    else rope_kernel<T, false><<<grid, RP_THREADS, 0, st>>>(c);
+// i / d = umulhi(i, ceil(2^32 / d)) for i and d below 2^16 (the items of a CTA)
+static unsigned divisor(int d) { return d == 1 ? 0u : (unsigned)((0x100000000ull + d - 1) / d); }
+
+template <typename T, int N>
+static int rope_launch(RopeCall &c, bool inter, cudaStream_t st) {
+    c.per = c.dims / 2 / N + (c.D - c.dims) / N;
+    // Few tokens: the heads of one over CTAs of up to two items a thread
+    // (latency). CTAs enough for all SMs several times over: all heads of a
+    // token in one, or of up to 4 tokens (its cosines are made once).
+    const int two = 2 * RP_THREADS;
+    c.tokens = 1;
+    c.hblock = c.heads;
+    if (c.n < 4 * num_sms()) {
+        const int hb = (c.heads * c.per + two - 1) / two;
+        c.hblock = (c.heads + hb - 1) / hb;
+    } else {
+        while (c.tokens < RP_MAXTOK && c.n / (c.tokens * 2) >= 4 * num_sms())
+            c.tokens *= 2;
+    }
+    if ((int64_t)c.tokens * c.hblock * c.per > 65535) c.hblock = 65535 / c.per;
+    const int hb = (c.heads + c.hblock - 1) / c.hblock;
+    c.per_mul = divisor(c.per);
+    c.h_mul = divisor(c.hblock);
+    dim3 grid((c.n + c.tokens - 1) / c.tokens, hb);
+    if (inter) rope_kernel<T, true, N><<<grid, RP_THREADS, 0, st>>>(c);
+    else rope_kernel<T, false, N><<<grid, RP_THREADS, 0, st>>>(c);
     MLXD_CHECK(cudaGetLastError());
     return 0;
 }
@@ -161,9 +228,11 @@ extern "C" int mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int he
     c.n = n;
     c.heads = heads;
     c.D = head_dim;
-    c.tokens = 1;
-    c.hblock = heads;
     const bool inter = r->interleaved != 0;
-    return dtype == MLXD_BF16 ? rope_launch<uint16_t>(c, inter, (cudaStream_t)stream)
-                              : rope_launch<float>(c, inter, (cudaStream_t)stream);
+    const int vec = dtype == MLXD_BF16 ? 8 : 4;
+    const bool whole = c.dims % (2 * vec) == 0 && (c.D - c.dims) % vec == 0 && ((uintptr_t)x & 15) == 0 &&
+                       ((uintptr_t)y & 15) == 0 && (c.xt | c.xh | c.yt | c.yh) % vec == 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == MLXD_BF16) return whole ? rope_launch<uint16_t, 8>(c, inter, st) : rope_launch<uint16_t, 1>(c, inter, st);
+    return whole ? rope_launch<float, 4>(c, inter, st) : rope_launch<float, 1>(c, inter, st);
 }
