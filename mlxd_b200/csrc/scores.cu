@@ -4,16 +4,18 @@
 //   M = max x,  S = sum_{i != argmax} e^(x_i - M),  W = sum (x_i - M) e^(x_i - M)
 //   logprob(t) = x_t - M - log1p(S),   H = log1p(S) - W / (1 + S)
 //
-// Bound by HBM: one pass reads every logit once. A thread keeps its largest
-// logit out of its own sums (so that a peaked row keeps its small terms), the
-// sums relative to a reference that moves only when the maximum has grown by
-// more than e^5. Merging thread, warp, CTA and cluster results rescales to the
-// common maximum and lets every held-out logit but the row's join.
-//
-// Top list: the k-th largest of the maxima of thread groups is a lower bound
-// T of the k-th largest logit, and no group below T holds any of the k; so
-// only k groups' logits (of 64) are read again, from L2, and what reaches T is
-// ranked by counting. Keys (value, index) are distinct, ties cost nothing.
+// Bound by HBM: one pass reads every logit once, and the arithmetic (an
+// exponential and some eight other instructions a logit) has to stay below
+// the issue rate. The first quarter of a CTA's logits sets the scene: every
+// thread keeps its largest logit out of its own sums, and T, the k-th largest
+// of the maxima of 64 thread groups, bounds the row's k-th largest logit from
+// below. From there on a logit that reaches T goes to a list in shared memory
+// (for random orders some 4 k of them), and all others are summed relative to
+// the first quarter's maximum, which they cannot exceed. At the end the kept
+// out logits but the largest join the sums (so a peaked row keeps its small
+// terms), and the list is ranked by counting; keys (value, index) are
+// distinct, ties cost nothing. A list that overflows (a row whose later
+// logits are the larger ones) is made again from the whole row's group maxima.
 #include "common.cuh"
 #include "kernels.h"
 
@@ -72,6 +74,29 @@ MLXD_DEV void sc_unpack(const uint4 &v, float (&x)[4]) {
 
 constexpr float SC_LOG2E = 1.4426950408889634f, SC_LN2 = 0.6931471805599453f;
 
+// two lanes of f32 in one instruction
+MLXD_DEV u64 pair2(float lo, float hi) {
+    u64 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+MLXD_DEV void unpair2(u64 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+MLXD_DEV u64 add2(u64 a, u64 b) {
+    u64 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+MLXD_DEV u64 mul2(u64 a, u64 b) {
+    u64 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+MLXD_DEV u64 fma2(u64 a, u64 b, u64 c) {
+    u64 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 // sums over what was seen but its largest logit: s of 2^z and w of z 2^z, z =
 // (x - ref) log2 e; best/at: the held-out logit (-inf: none above -inf yet)
 struct ScoreSums {
@@ -79,6 +104,35 @@ struct ScoreSums {
     int at;
 };
 
+// logits that do not exceed ref by much: -inf counts 2^-200 = 0, NaN stays NaN
+template <int N>
+MLXD_DEV void sc_sum(ScoreSums &a, const float (&x)[N]) {
+    if constexpr (N == 1) {
+        const float z = max_nan((x[0] - a.ref) * SC_LOG2E, -200.f), e = sc_ex2(z);
+        a.s += e;
+        a.w = fmaf(z, e, a.w);
+    } else {
+        const u64 ref2 = pair2(-a.ref, -a.ref), log2e2 = pair2(SC_LOG2E, SC_LOG2E);
+        u64 s2 = pair2(a.s, 0.f), w2 = pair2(a.w, 0.f);
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            float z0, z1;
+            unpair2(mul2(add2(pair2(x[i], x[i + 1]), ref2), log2e2), z0, z1);
+            z0 = max_nan(z0, -200.f);
+            z1 = max_nan(z1, -200.f);
+            const u64 e = pair2(sc_ex2(z0), sc_ex2(z1));
+            s2 = add2(s2, e);
+            w2 = fma2(pair2(z0, z1), e, w2);
+        }
+        float t;
+        unpair2(s2, a.s, t);
+        a.s += t;
+        unpair2(w2, a.w, t);
+        a.w += t;
+    }
+}
+
+// any logits: a larger one than before is held out in place of the old
 template <int N>
 MLXD_DEV void sc_add(ScoreSums &a, float (&x)[N], int base) {
     float mx = x[0];
@@ -89,8 +143,10 @@ MLXD_DEV void sc_add(ScoreSums &a, float (&x)[N], int base) {
 #pragma unroll
         for (int i = N - 2; i >= 0; i--) j = x[i] == mx ? i : j;
         const bool first = a.best == -INFINITY;
-        if (first || mx > a.ref + 5.0f) {
-            const float d = first ? 0.f : (a.ref - mx) * SC_LOG2E, f = sc_ex2(d);
+        if (first && a.s == 0.f) {
+            a.ref = mx;
+        } else if (mx > a.ref + 5.0f) {
+            const float d = (a.ref - mx) * SC_LOG2E, f = sc_ex2(d);
             a.w = f * fmaf(d, a.s, a.w);
             a.s *= f;
             a.ref = mx;
@@ -105,13 +161,7 @@ MLXD_DEV void sc_add(ScoreSums &a, float (&x)[N], int base) {
 #pragma unroll
         for (int i = 0; i < N; i++) x[i] = i == j ? -INFINITY : x[i];
     }
-    // -inf counts 2^-200 = 0; NaN stays NaN
-#pragma unroll
-    for (int i = 0; i < N; i++) {
-        const float z = max_nan((x[i] - a.ref) * SC_LOG2E, -200.f), e = sc_ex2(z);
-        a.s += e;
-        a.w = fmaf(z, e, a.w);
-    }
+    sc_sum<N>(a, x);
 }
 
 // (s, w) relative to ref, expressed relative to m >= ref's row maximum
@@ -141,13 +191,21 @@ MLXD_DEV u64 ld_cluster64(const u64 *p, int rank) {
     return v;
 }
 
+// the largest logit of a vector (NaN aside)
+MLXD_DEV float sc_max(const uint4 &v, const float (&)[8]) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+MLXD_DEV float sc_max(const uint4 &, const float (&x)[4]) { return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])); }
+
 template <typename T>
 __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_constant__ ScoreCall c) {
     constexpr int N = 16 / sizeof(T), NWARP = SC_THREADS / 32;
     __shared__ ScorePart part;
     __shared__ u64 s_wkey[NWARP], s_gkey[SC_GROUPS], s_cand[SC_CAND], s_t;
     __shared__ float s_ws[NWARP][2];
-    __shared__ int s_flag[SC_GROUPS], s_nflag, s_ncand;
+    __shared__ int s_flag[SC_THREADS], s_nflag, s_ncand;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int rank = blockIdx.x, ncta = gridDim.x;   // the cluster spans x
     const int64_t row = blockIdx.y + (int64_t)blockIdx.z * 65535;
@@ -160,21 +218,100 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + head);
     const int extras = rank == 0 ? head + c.V - tail0 : 0;
     auto extra_at = [&](int i) { return i < head ? i : tail0 + i - head; };
+    const int want = max(c.top, 4);                  // T's rank
 
+    auto warp_max64 = [&](u64 k) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, k, o);
+            k = other > k ? other : k;
+        }
+        return k;
+    };
+    auto block_max64 = [&](u64 k) {                  // two barriers
+        k = warp_max64(k);
+        __syncthreads();
+        if (lane == 0) s_wkey[warp] = k;
+        __syncthreads();
+        k = s_wkey[0];
+#pragma unroll
+        for (int w = 1; w < NWARP; w++) k = s_wkey[w] > k ? s_wkey[w] : k;
+        return k;
+    };
+    // f(list[i], how many of list[0 .. n) are larger) for every i, a thread each
+    auto ranks = [&](const u64 *list, int n, auto f) {
+        for (int i = tid; i < n; i += SC_THREADS) {
+            const u64 k = list[i];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < n; j++) above += list[j] > k;
+            f(k, above);
+        }
+    };
+    // From the threads' largest keys over vectors [v0, ve) (and the extras):
+    // T into s_t (1: fewer than `want` groups hold anything above -inf), and
+    // what reaches T appended to s_cand. The threads' own keys are flagged
+    // against T, so that some `want` threads' logits are read again.
+    auto collect = [&](u64 mine, int ve) {
+        u64 q = mine;
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            const u64 other = __shfl_xor_sync(0xffffffffu, q, o);
+            q = other > q ? other : q;
+        }
+        __syncthreads();
+        if ((lane & 3) == 0) s_gkey[tid >> 2] = q;
+        if (tid == 0) {
+            s_t = 1ull;
+            s_nflag = 0;
+        }
+        __syncthreads();
+        ranks(s_gkey, SC_GROUPS, [&](u64 g, int above) {
+            if (g && above == want - 1) s_t = g;
+        });
+        __syncthreads();
+        const u64 t = s_t;
+        if (mine >= t) s_flag[atomicAdd(&s_nflag, 1)] = tid;
+        __syncthreads();
+        auto offer = [&](float v, int i) {
+            if (!(v > -INFINITY)) return;
+            const u64 k = sc_key(v, i);
+            if (k < t) return;
+            const int at = atomicAdd(&s_ncand, 1);
+            if (at < SC_CAND) s_cand[at] = k;
+        };
+        // (flagged thread, round) over all threads: the loads of a list go out together
+        const int nflag = s_nflag, per = (ve - v0 + SC_THREADS - 1) / SC_THREADS;
+        for (int i = tid; i < nflag * per; i += SC_THREADS) {
+            const int f = i / per, v = v0 + s_flag[f] + (i - f * per) * SC_THREADS;
+            if (v >= ve) continue;
+            float e[N];
+            sc_unpack(ldg_nc_v4(xv + v), e);
+#pragma unroll
+            for (int j = 0; j < N; j++) offer(e[j], head + v * N + j);
+        }
+        if (mine >= t && tid < extras) offer(sc_load(x, extra_at(tid)), extra_at(tid));
+        __syncthreads();
+        return t;
+    };
+
+    if (tid == 0) s_ncand = 0;
+    const int target = tid == 0 && rank == 0 && c.lp ? c.targets[row] : -1;
+    // the first quarter
     ScoreSums a = {0.f, 0.f, 0.f, -INFINITY, 0};
-    // in index order, so that a thread holds out the first of equal logits
-    if (tid < min(head, extras)) {
+    const int rounds = (v1 - v0 + SC_THREADS - 1) / SC_THREADS, va = min(v1, v0 + (rounds + 3) / 4 * SC_THREADS);
+    if (tid < min(head, extras)) {                   // in index order: a thread holds out the first of equal logits
         float e[1] = {sc_load(x, tid)};
         sc_add<1>(a, e, tid);
     }
-    for (int v = v0 + tid; v < v1; v += SC_UNROLL * SC_THREADS) {
+    for (int v = v0 + tid; v < va; v += SC_UNROLL * SC_THREADS) {
         uint4 u[SC_UNROLL];
 #pragma unroll
         for (int k = 0; k < SC_UNROLL; k++)
-            if (v + k * SC_THREADS < v1) u[k] = ldg_nc_v4(xv + v + k * SC_THREADS);
+            if (v + k * SC_THREADS < va) u[k] = ldg_nc_v4(xv + v + k * SC_THREADS);
 #pragma unroll
         for (int k = 0; k < SC_UNROLL; k++)
-            if (v + k * SC_THREADS < v1) {
+            if (v + k * SC_THREADS < va) {
                 float e[N];
                 sc_unpack(u[k], e);
                 sc_add<N>(a, e, head + (v + k * SC_THREADS) * N);
@@ -184,41 +321,74 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
         float e[1] = {sc_load(x, extra_at(tid))};
         sc_add<1>(a, e, extra_at(tid));
     }
+    const float xt = target >= 0 && target < c.V ? sc_load(x, target) : 0.f;   // on its way until the end
+    u64 mine = a.best > -INFINITY ? sc_key(a.best, a.at) : 0ull;
+    const u64 t0 = collect(mine, va);
+    const int na = s_ncand;                          // listed and already summed or kept out
+
+    // the rest
+    if (va < v1) {
+        const u64 key = block_max64(mine);
+        const float ma = key ? sc_val(key) : 0.f, tv = t0 > 1 ? sc_val(t0) : -3.4028235e38f;
+        if (a.best > -INFINITY) sc_move(a.s, a.w, a.ref, ma);
+        a.ref = ma;
+        auto add = [&](const uint4 &u, int v) {
+            float e[N];
+            sc_unpack(u, e);
+            if (sc_max(u, e) >= tv) {
+                unsigned hit = 0;
+                bool room = true;
+#pragma unroll
+                for (int j = 0; j < N; j++) hit |= e[j] >= tv ? 1u << j : 0u;
+                int at = atomicAdd(&s_ncand, __popc(hit));
+                if (at + __popc(hit) <= SC_CAND) {
+#pragma unroll
+                    for (int j = 0; j < N; j++)
+                        if (hit >> j & 1) {
+                            s_cand[at++] = sc_key(e[j], head + v * N + j);
+                            e[j] = -INFINITY;
+                        }
+                } else {
+                    for (; at < SC_CAND; at++) s_cand[at] = 0ull;   // reserved, left empty
+                    room = false;
+                }
+                if (!room) {                         // kept out as in the first quarter
+                    sc_add<N>(a, e, head + v * N);
+                    return;
+                }
+            }
+            sc_sum<N>(a, e);
+        };
+        for (int v = va + tid; v < v1; v += SC_UNROLL * SC_THREADS) {
+            uint4 u[SC_UNROLL];
+#pragma unroll
+            for (int k = 0; k < SC_UNROLL; k++)
+                if (v + k * SC_THREADS < v1) u[k] = ldg_nc_v4(xv + v + k * SC_THREADS);
+#pragma unroll
+            for (int k = 0; k < SC_UNROLL; k++)
+                if (v + k * SC_THREADS < v1) add(u[k], v + k * SC_THREADS);
+        }
+    }
+    __syncthreads();
+    const int nc = s_ncand, listed = min(nc, SC_CAND);
 
     // the CTA's largest logit and the sums of the rest
-    const u64 mine = a.best > -INFINITY ? sc_key(a.best, a.at) : 0ull;
-    u64 k1 = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const u64 other = __shfl_xor_sync(0xffffffffu, k1, o);
-        k1 = other > k1 ? other : k1;
-        if (o == 2 && (lane & 3) == 0) s_gkey[tid >> 2] = k1;
-    }
-    if (lane == 0) s_wkey[warp] = k1;
-    if (tid == 0) s_nflag = s_ncand = 0;
-    __syncthreads();
-    u64 key = s_wkey[0];
-#pragma unroll
-    for (int w = 1; w < NWARP; w++) key = s_wkey[w] > key ? s_wkey[w] : key;
-    const float m = key ? sc_val(key) : -INFINITY;
-    if (a.best > -INFINITY) {
+    mine = a.best > -INFINITY ? sc_key(a.best, a.at) : 0ull;
+    u64 key = mine;
+    for (int i = tid; i < listed; i += SC_THREADS) key = s_cand[i] > key ? s_cand[i] : key;
+    key = block_max64(key);
+    if (key) {
+        const float m = sc_val(key);
         sc_move(a.s, a.w, a.ref, m);
-        if (mine != key) sc_join(a.s, a.w, a.best, m);
+        if (mine && mine != key) sc_join(a.s, a.w, a.best, m);
+        for (int i = na + tid; i < listed; i += SC_THREADS)
+            if (s_cand[i] && s_cand[i] != key) sc_join(a.s, a.w, sc_val(s_cand[i]), m);
     }
     a.s = warp_sum(a.s);
     a.w = warp_sum(a.w);
     if (lane == 0) {
         s_ws[warp][0] = a.s;
         s_ws[warp][1] = a.w;
-    }
-    // T: the top-th largest group maximum (all above -inf when there are fewer)
-    if (c.top && tid < SC_GROUPS) {
-        const u64 g = s_gkey[tid];
-        int above = 0;
-#pragma unroll 8
-        for (int i = 0; i < SC_GROUPS; i++) above += s_gkey[i] > g;
-        if (g && above < c.top) s_flag[atomicAdd(&s_nflag, 1)] = tid;
-        if (g && above == c.top - 1) s_t = g;
     }
     __syncthreads();
     if (tid == 0) {
@@ -232,70 +402,41 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
         part.w = w;
     }
     if (c.top) {
-        const int nflag = s_nflag;
-        const u64 T0 = nflag == c.top ? s_t : 1ull;
-        const float tv = nflag == c.top ? sc_val(T0) : -INFINITY;
-        auto offer = [&](float v, int i) {
-            if (v >= tv && v > -INFINITY) {
-                const u64 k = sc_key(v, i);
-                if (k >= T0) {
-                    const int at = atomicAdd(&s_ncand, 1);
-                    if (at < SC_CAND) s_cand[at] = k;
-                }
-            }
-        };
-        for (int f = warp; f < nflag; f += NWARP) {
-            const int g = s_flag[f];
-            for (int i = lane;; i += 32) {
-                const int v = v0 + 4 * g + (i & 3) + (i >> 2) * SC_THREADS;
-                if (v - (i & 3) >= v1) break;
-                if (v >= v1) continue;
+        int n = nc;
+        // every logit above -inf of this CTA, as a key, to f
+        auto each = [&](auto f) {
+            if (tid < extras) f(sc_load(x, extra_at(tid)), extra_at(tid));
+            for (int v = v0 + tid; v < v1; v += SC_THREADS) {
                 float e[N];
                 sc_unpack(ldg_nc_v4(xv + v), e);
 #pragma unroll
-                for (int j = 0; j < N; j++) offer(e[j], head + v * N + j);
+                for (int j = 0; j < N; j++) f(e[j], head + v * N + j);
             }
-            if (lane < 4 && 4 * g + lane < extras) offer(sc_load(x, extra_at(4 * g + lane)), extra_at(4 * g + lane));
+        };
+        if (n > SC_CAND) {                           // again, with the whole row's group maxima
+            u64 b = 0;
+            each([&](float v, int i) {
+                if (v > -INFINITY) b = max(b, sc_key(v, i));
+            });
+            if (tid == 0) s_ncand = 0;
+            collect(b, v1);
+            n = s_ncand;
         }
-        __syncthreads();
-        const int nc = s_ncand;
-        if (nc <= SC_CAND) {
-            for (int i = tid; i < nc; i += SC_THREADS) {
-                const u64 k = s_cand[i];
-                int above = 0;
-                for (int j = 0; j < nc; j++) above += s_cand[j] > k;
+        if (n <= SC_CAND) {
+            ranks(s_cand, n, [&](u64 k, int above) {
                 if (above < c.top) part.list[above] = k;
-            }
-            if (tid == 0) part.count = min(nc, c.top);
+            });
+            if (tid == 0) part.count = min(n, c.top);
         } else {
-            // more reach T than there is room for (k groups that hold nearly all of the largest): the
-            // largest below the last one, again and again
+            // a few threads hold nearly all of the largest: the largest below the last one, again and again
             u64 last = ~0ull;
             for (int r = 0; r < c.top; r++) {
                 u64 b = 0;
-                auto look = [&](float v, int i) {
-                    if (v > -INFINITY) {
-                        const u64 k = sc_key(v, i);
-                        b = k < last && k > b ? k : b;
-                    }
-                };
-                if (tid < extras) look(sc_load(x, extra_at(tid)), extra_at(tid));
-                for (int v = v0 + tid; v < v1; v += SC_THREADS) {
-                    float e[N];
-                    sc_unpack(ldg_nc_v4(xv + v), e);
-#pragma unroll
-                    for (int j = 0; j < N; j++) look(e[j], head + v * N + j);
-                }
-#pragma unroll
-                for (int o = 16; o; o >>= 1) {
-                    const u64 other = __shfl_xor_sync(0xffffffffu, b, o);
-                    b = other > b ? other : b;
-                }
-                __syncthreads();
-                if (lane == 0) s_wkey[warp] = b;
-                __syncthreads();
-                last = 0;
-                for (int w = 0; w < NWARP; w++) last = s_wkey[w] > last ? s_wkey[w] : last;
+                each([&](float v, int i) {
+                    const u64 k = v > -INFINITY ? sc_key(v, i) : 0ull;
+                    if (k < last) b = max(b, k);
+                });
+                last = block_max64(b);
                 if (tid == 0) part.list[r] = last;
             }
             if (tid == 0) part.count = c.top;
@@ -342,14 +483,24 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
             s_m = M;
             s_ls = ls;
             s_ent = empty ? 0.f : ls - w * SC_LN2 / (1.f + s);
-            s_count = 0;
         }
     }
+    // the parts' lists: what is above the last entry of a full one
     if (c.top && ncta > 1) {
-        for (int i = tid; i < ncta * c.top; i += SC_THREADS) {
-            const int k = i / c.top, j = i - k * c.top;
-            int n = (int)__float_as_uint(ld_cluster(reinterpret_cast<const float *>(&part.count), k));
-            s_cand[i] = j < n ? ld_cluster64(&part.list[j], k) : 0ull;
+        u64 full = 0;
+        if (lane < ncta) {
+            const int n = (int)__float_as_uint(ld_cluster(reinterpret_cast<const float *>(&part.count), lane));
+            if (n == c.top) full = ld_cluster64(&part.list[n - 1], lane);
+            if (warp == 0) s_flag[lane] = n;
+        }
+        full = warp_max64(full);
+        if (tid == 0) s_ncand = 0;
+        __syncthreads();
+        for (int i = tid; i < ncta * SC_TOP; i += SC_THREADS) {
+            const int k = i / SC_TOP, j = i % SC_TOP;
+            if (j >= s_flag[k]) continue;
+            const u64 v = ld_cluster64(&part.list[j], k);
+            if (v >= full) s_cand[atomicAdd(&s_ncand, 1)] = v;
         }
     }
     __syncthreads();
@@ -357,23 +508,16 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
     const float M = s_m, ls = s_ls;
     const bool empty = M == -INFINITY && !isnan(ls);
     if (tid == 0) {
-        if (c.lp) {
-            const int t = c.targets[row];
-            c.lp[row] = t < 0 || t >= c.V ? __int_as_float(0x7fc00000) : empty ? -INFINITY : sc_load(x, t) - M - ls;
-        }
+        if (c.lp)
+            c.lp[row] = target < 0 || target >= c.V ? __int_as_float(0x7fc00000) : empty ? -INFINITY : xt - M - ls;
         if (c.ent) c.ent[row] = s_ent;
     }
     if (!c.top) return;
     if (ncta > 1) {
-        for (int i = tid; i < ncta * c.top; i += SC_THREADS) {
-            const u64 k = s_cand[i];
-            int above = 0;
-            for (int j = 0; j < ncta * c.top; j++) above += s_cand[j] > k;
-            if (k && above < c.top) {
-                s_list[above] = k;
-                atomicAdd(&s_count, 1);
-            }
-        }
+        ranks(s_cand, s_ncand, [&](u64 k, int above) {
+            if (above < c.top) s_list[above] = k;
+        });
+        if (tid == 0) s_count = min(s_ncand, c.top);
     } else {
         if (tid < part.count) s_list[tid] = part.list[tid];
         if (tid == 0) s_count = part.count;
@@ -411,7 +555,7 @@ static int launch_scores(const ScoreCall &c, cudaStream_t st) {
     auto kern = scores_kernel<T>;
     // few rows: a cluster per row while there are SMs and every thread keeps a vector
     int cl = 1;
-    while (cl < SC_MAXCL && (int64_t)c.rows * cl * 2 <= num_sms() && c.V > cl * SC_THREADS * (int)(16 / sizeof(T))) cl *= 2;
+    while (cl < SC_MAXCL && (int64_t)c.rows * cl * 2 <= num_sms() && c.V > 4 * cl * SC_THREADS * (int)(16 / sizeof(T))) cl *= 2;
     if (cl > 8 && !nonportable_allowed((const void *)kern)) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(cl, c.rows < 65535 ? c.rows : 65535, (c.rows + 65534) / 65535);

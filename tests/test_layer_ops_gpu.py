@@ -261,6 +261,32 @@ def test_scores_hard_rows(gen, V, kind, dtype):
     scores_check(o, x, t, top)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows", [2, 80])
+@pytest.mark.parametrize("kind", ["late", "rising", "strided", "few late", "gaps"])
+def test_scores_rows_ordered_against_the_scan(gen, kind, rows, dtype):
+    """Rows whose largest logits come late, rise along the row, lie where a few threads read, or are the only ones."""
+    V = 70001
+    x = rand(gen, rows, V, dtype=torch.float32)
+    at = torch.arange(V, device="cuda")
+    if kind == "late":
+        x[:, :V // 3] = -math.inf
+    elif kind == "rising":
+        x += at * 1e-3
+    elif kind == "strided":
+        n = 8 if dtype == torch.bfloat16 else 4
+        x[:, (at // n) % 256 < 3] += 9.0
+    elif kind == "gaps":        # threads that see nothing above -inf until late, then a rising rest
+        n = 8 if dtype == torch.bfloat16 else 4
+        x[:, ((at // n) % 256 % 4 < 3) & (at < V // 2)] = -math.inf
+        x += at * 1e-4
+    else:
+        x[:, :V - 40] = -math.inf
+    x = x.to(dtype)
+    t = torch.randint(0, V, (rows,), device="cuda", generator=gen).to(torch.int32)
+    scores_check(scores_call(x, t, 20), x, t, 20)
+
+
 def test_scores_peaked_rows_keep_their_small_terms(gen):
     """A row whose other tokens hold 1e-12 of the mass: entropy and logprob to f32 precision of themselves."""
     V = 3001
