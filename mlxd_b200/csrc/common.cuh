@@ -21,6 +21,13 @@ MLXD_DEV float rbf(float f) { return bf2f(f2bf(f)); }
 MLXD_DEV uint32_t pack_bf2(float lo, float hi) {
     return (uint32_t)f2bf(lo) | ((uint32_t)f2bf(hi) << 16);
 }
+// the same rounding of two values in one conversion (single ones run on the
+// quarter-rate pipe that exponentials need)
+MLXD_DEV uint32_t cvt_bf2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 MLXD_DEV float lo_bf(uint32_t v) { return __uint_as_float(v << 16); }
 MLXD_DEV float hi_bf(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
@@ -224,6 +231,29 @@ MLXD_DEV unsigned smid_() {
 // consumer grid be scheduled. No-ops when the launch has no PDL attribute.
 MLXD_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 MLXD_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ---- two lanes of f32 in one instruction
+MLXD_DEV uint64_t pair2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+MLXD_DEV void unpair2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+MLXD_DEV uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+MLXD_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+MLXD_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 
 // ---- clusters: barrier over all CTAs, and loads of CTA `rank`'s shared memory
 MLXD_DEV void cluster_sync_all() {

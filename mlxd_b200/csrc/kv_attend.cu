@@ -290,9 +290,9 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
             for (int t = 0; t < 2; t++) {
                 const float e0 = exp2f((z[t][x] - mu) * s2), e1 = exp2f((z[t][x + 1] - mu) * s2);
                 l += e0 + e1;
-                const uint32_t h = pack_bf2(e0, e1);
+                const uint32_t h = cvt_bf2(e0, e1);
                 ph[2 * t + x / 2] = h;
-                pl[2 * t + x / 2] = pack_bf2(e0 - lo_bf(h), e1 - hi_bf(h));
+                pl[2 * t + x / 2] = cvt_bf2(e0 - lo_bf(h), e1 - hi_bf(h));
             }
         };
         half(0, m0, l0);
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
         }
         const float inv = M == -INFINITY ? 0.f : 1.0f / L;   // a row that sees nothing is zero
         *reinterpret_cast<uint2 *>(c.out + token * c.out_stride + (int64_t)qh * c.D + d) =
-            make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+            make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
     }
     cluster_sync_all();                            // no CTA leaves while its shared memory is read
 }
@@ -481,6 +481,9 @@ static int attend_few(const AttnCall &c, int rows, int keys, bool pdl, cudaStrea
 // Keys no row of the CTA sees may hold anything: their scores are masked and
 // their value rows zeroed in shared memory. Every wait is bounded; a launch
 // that gave up says so in a host word that the next call reports.
+#ifndef AT_POLY
+#define AT_POLY 0
+#endif
 constexpr int AT_THREADS = 384, AT_KT = 128, AT_ROWS = 256;
 
 template <int DB>
@@ -512,6 +515,23 @@ MLXD_DEV float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 2^x on the FMA pipe for two x <= 127: nearest integer n by adding 1.5 2^23,
+// a cubic for 2^(x - n) on [-1/2, 1/2] (relative error 7.5e-5, minimax fit;
+// the weights are rounded to 2^-9), n into the exponent. Below 2^-125: 2^-125.
+MLXD_DEV void ex2_pair(float &x0, float &x1) {
+    const uint64_t magic = pair2(12582912.f, 12582912.f), neg = pair2(-12582912.f, -12582912.f);
+    const uint64_t x = pair2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+    const uint64_t t = add2(x, magic);
+    const uint64_t n = add2(t, neg), f = fma2(n, pair2(-1.f, -1.f), x);
+    uint64_t p = fma2(f, pair2(5.517155e-2f, 5.517155e-2f), pair2(0.24261136f, 0.24261136f));
+    p = fma2(f, p, pair2(0.69326102f, 0.69326102f));
+    p = fma2(f, p, pair2(0.99992806f, 0.99992806f));
+    float p0, p1, t0, t1;
+    unpair2(p, p0, p1);
+    unpair2(t, t0, t1);
+    x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
+    x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
+}
 
 template <int DB>
 __global__ void __launch_bounds__(AT_THREADS, 1)
@@ -523,7 +543,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     unsigned char *sm = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *kfull = reinterpret_cast<uint64_t *>(sm + L::BARS);
     uint64_t *kempty = kfull + NS, *vfull = kempty + NS, *vempty = vfull + NS;
-    uint64_t *sfull = vempty + NS, *pfull = sfull + 2, *odone = pfull + 2;
+    uint64_t *sfull = vempty + NS, *pfull = sfull + 2, *odone = pfull + 4;   // pfull[2 t + half]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(odone + 1);
     __shared__ int s_pmin, s_pmax, s_fail;
 
@@ -538,10 +558,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             mbar_init(&vfull[i], 1);
             mbar_init(&vempty[i], 1);
         }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&sfull[i], 1);
-            mbar_init(&pfull[i], 4);
-        }
+        for (int i = 0; i < 2; i++) mbar_init(&sfull[i], 1);
+        for (int i = 0; i < 4; i++) mbar_init(&pfull[i], 4);
         mbar_init(odone, 1);
         s_pmin = INT32_MAX;
         s_pmax = -1;
@@ -602,8 +620,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         return k * AT_KT;
     };
 
-    if (warp == 0) {
-        if (lane == 0) {
+    // registers to the softmax warps: 128 x (72 + 2 x 208) of the block's 384 x 168
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0 && lane == 0) {
             const uint64_t mk = reinterpret_cast<uint64_t>(&tmk), mv = reinterpret_cast<uint64_t>(&tmv);
             int kn = 0, vn = 0;                      // loads issued
             bool ok = true;
@@ -631,66 +651,64 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 if (kn > i) mbar_wait(&kfull[(kn - 1 - i) % NS], ((kn - 1 - i) / NS) & 1);
                 if (vn > i) mbar_wait(&vfull[(vn - 1 - i) % NS], ((vn - 1 - i) / NS) & 1);
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && j1 > j0) {
+        } else if (warp == 1 && j1 > j0) {
             constexpr uint32_t iqk = umma_idesc_bf16(128, AT_KT, false), ipv = umma_idesc_bf16(128, DB * 64, true);
-            const uint32_t q0 = smem_u32(sm + L::Q), k0 = smem_u32(sm + L::K), v0 = smem_u32(sm + L::V);
+            const uint64_t qd = umma_desc_sw128(smem_u32(sm + L::Q)), kd = umma_desc_sw128(smem_u32(sm + L::K));
+            const uint64_t vd = umma_desc_sw128_mn(smem_u32(sm + L::V), L::BLOCK);
             auto qk = [&](int i, int n) {            // S_i = Q_i K_n^T
-                const uint32_t kt = k0 + (n % NS) * L::TILE, qt = q0 + i * L::TILE;
+                const uint64_t qt = qd + i * (L::TILE >> 4), kt = kd + (n % NS) * (L::TILE >> 4);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < DB * 4; k++) {
-                    const uint32_t off = (k >> 2) * L::BLOCK + (k & 3) * 32;
-                    asm volatile(
-                        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem + i * 128),
-                        "l"(umma_desc_sw128(qt + off)), "l"(umma_desc_sw128(kt + off)), "r"(iqk), "r"(k)
-                        : "memory");
-                }
-            };
-            auto pv = [&](int i, int n) {            // O_i += P_i V_n
-                const uint32_t vt = v0 + (n % NS) * L::TILE;
-#pragma unroll
-                for (int k = 0; k < AT_KT / 16; k++)
-                    asm volatile(
-                        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem + 256 + i * 128),
-                        "r"(tmem + i * 128 + k * 8), "l"(umma_desc_sw128_mn(vt + k * 2048, L::BLOCK)), "r"(ipv),
-                        "r"(n + k)
-                        : "memory");
-            };
-            const int nn = j1 - j0;
-            bool ok = mbar_wait(&kfull[0], 0);
-            if (ok) {
-                tc_fence_after();
-                for (int i = 0; i < nq; i++) {
-                    qk(i, 0);
+                    for (int k = 0; k < DB * 4; k++) {
+                        const uint64_t off = ((k >> 2) * L::BLOCK + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + i * 128, qt + off, kt + off, iqk, k != 0);
+                    }
                     tc_commit(&sfull[i]);
                 }
-                tc_commit(&kempty[0]);
+            };
+            auto pv = [&](int i, int n, int half) {  // O_i += P_i V_n over 64 keys
+                const uint64_t vt = vd + (n % NS) * (L::TILE >> 4) + half * (4 * 2048 >> 4);
+                const uint32_t pt = tmem + i * 128 + half * 32;
+                if (elect_one())
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        mma_ts(tmem + 256 + i * 128, pt + k * 8, vt + (k * 2048 >> 4), ipv, n + half + k != 0);
+            };
+            auto release = [&](uint64_t *bar) {
+                if (elect_one()) tc_commit(bar);
+            };
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+                tc_fence_after();
+                return got;
+            };
+            const int nn = j1 - j0;
+            bool ok = wait(&kfull[0], 0);
+            if (ok) {
+                for (int i = 0; i < nq; i++) qk(i, 0);
+                release(&kempty[0]);
             }
+            // the query tiles strictly in turn, which keeps one in its softmax while the other multiplies
             for (int n = 0; n < nn && ok; n++) {
                 for (int i = 0; i < nq && ok; i++) {
-                    if (i == 0) ok = mbar_wait(&vfull[n % NS], (n / NS) & 1);
-                    ok = ok && mbar_wait(&pfull[i], n & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    pv(i, n);
-                    if (n + 1 < nn) {
-                        if (i == 0) ok = mbar_wait(&kfull[(n + 1) % NS], ((n + 1) / NS) & 1);
+                    if (i == 0) ok = wait(&vfull[n % NS], (n / NS) & 1);
+                    for (int h = 0; h < 2 && ok; h++)
+                        if ((ok = wait(&pfull[2 * i + h], n & 1))) pv(i, n, h);
+                    if (ok && n + 1 < nn) {
+                        if (i == 0) ok = wait(&kfull[(n + 1) % NS], ((n + 1) / NS) & 1);
                         if (!ok) break;
-                        tc_fence_after();
                         qk(i, n + 1);
-                        tc_commit(&sfull[i]);
-                        if (i == nq - 1) tc_commit(&kempty[(n + 1) % NS]);
+                        if (i == nq - 1) release(&kempty[(n + 1) % NS]);
                     }
-                    if (i == nq - 1) tc_commit(&vempty[n % NS]);
+                    if (i == nq - 1) release(&vempty[n % NS]);
                 }
             }
-            tc_commit(odone);
-            if (!mbar_wait(odone, 0) || !ok) s_fail = 1;
+            release(odone);
+            if (!wait(odone, 0) || !ok) s_fail = 1;
         }
-    } else if (warp >= 4 && (warp - 4) / 4 < nq) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        if ((warp - 4) / 4 < nq) {
         const int wg = (warp - 4) >> 2, row = r0 + wg * 128 + (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
@@ -700,7 +718,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         // what this row sees; rows that are not asked for see all (and are dropped)
         Span sp = {0, 0, 0, 0, INT32_MAX};
         if (p >= 0) sp = span_of(c, window_lo(c, p), p + 1);
-        float m = -INFINITY, l = 0.f;
+        float m = -INFINITY;
+        uint64_t l[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};   // the row sum, in four
         bool ok = true;
         for (int n = 0; n < j1 - j0; n++) {
             const int s0 = tile_slot(j0 + n);
@@ -718,54 +737,41 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 break;
             }
             tc_fence_after();
-            uint32_t v[32];
-            float mx = -INFINITY;
+            uint32_t v[4][32];
+#pragma unroll
+            for (int w = 0; w < 4; w++) tmem_ld32(v[w], ts + 32 * w);
+            tmem_wait_ld();
+            if (!whole)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+#pragma unroll
+                    for (int x = 0; x < 32; x++) v[w][x] = see[w] >> x & 1 ? v[w][x] : 0xff800000u;
+            float mw[4];
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                tmem_ld32(v, ts + 32 * w);
-                tmem_wait_ld();
-                if (whole) {
+                mw[w] = __uint_as_float(v[w][0]);
 #pragma unroll
-                    for (int x = 0; x < 32; x++) mx = fmaxf(mx, __uint_as_float(v[x]));
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 32; x++) mx = fmaxf(mx, see[w] >> x & 1 ? __uint_as_float(v[x]) : -INFINITY);
-                }
+                for (int x = 1; x < 32; x++) mw[w] = fmaxf(mw[w], __uint_as_float(v[w][x]));
             }
+            const float mx = fmaxf(fmaxf(mw[0], mw[1]), fmaxf(mw[2], mw[3]));
             // a new maximum only when the old one is too far below
             const bool grow = mx > m + slack || (m == -INFINITY && mx > -INFINITY);
             if (__any_sync(0xffffffffu, grow)) {
                 const float a = grow ? ex2((m - mx) * s2) : 1.0f;
                 if (grow) m = mx;
-                l *= a;
+                l[0] = mul2(l[0], pair2(a, a));
+                l[1] = mul2(l[1], pair2(a, a));
                 if (n > 0)
 #pragma unroll
-                    for (int w = 0; w < DB * 2; w++) {
-                        tmem_ld32(v, to + 32 * w);
+                    for (int w = 0; w < DB * 4; w++) {
+                        uint32_t o[16];
+                        tmem_ld16(o, to + 16 * w);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * a);
-                        tmem_st32(to + 32 * w, v);
+                        for (int x = 0; x < 16; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * a);
+                        tmem_st16(to + 16 * w, o);
                     }
             }
-            const float mu = m == -INFINITY ? 0.f : m * s2;
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                tmem_ld32(v, ts + 32 * w);
-                tmem_wait_ld();
-                if (!whole)
-#pragma unroll
-                    for (int x = 0; x < 32; x++) v[x] = see[w] >> x & 1 ? v[x] : 0xff800000u;
-                uint32_t pk[16];
-#pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    pk[x] = pack_bf2(ex2(fmaf(__uint_as_float(v[2 * x]), s2, -mu)),
-                                     ex2(fmaf(__uint_as_float(v[2 * x + 1]), s2, -mu)));
-                    l += lo_bf(pk[x]) + hi_bf(pk[x]);
-                }
-                tmem_st16(ts + 16 * w, pk);
-            }
-            tmem_wait_st();
             // value rows of slots that no row sees: whatever they hold must not meet a zero weight
             if (wg == 0 && !(s0 >= all.b0 && s0 + AT_KT <= all.b1)) {
                 if (!__all_sync(0xffffffffu, mbar_wait(&vfull[n % NS], (n / NS) & 1))) {
@@ -783,9 +789,37 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                                 make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[wg]);
+            const float mu = m == -INFINITY ? 0.f : m * s2;
+            const uint64_t ss = pair2(s2, s2), mm = pair2(-mu, -mu);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int x = 0; x < 32; x++) {
+                    const int w = 2 * h + x / 16, y = 2 * (x % 16);
+                    float e0, e1;
+                    unpair2(fma2(pair2(__uint_as_float(v[w][y]), __uint_as_float(v[w][y + 1])), ss, mm), e0, e1);
+                    if (AT_POLY && x % (AT_POLY + !AT_POLY) == AT_POLY - 1) {
+                        ex2_pair(e0, e1);
+                    } else {
+                        e0 = ex2(e0);
+                        e1 = ex2(e1);
+                    }
+                    pk[x] = cvt_bf2(e0, e1);
+                    l[x & 1] = add2(l[x & 1], pair2(lo_bf(pk[x]), hi_bf(pk[x])));
+                }
+                tmem_st32(ts + 32 * h, pk);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[2 * wg + h]);
+            }
+        }
+        float lsum;
+        {
+            float t;
+            unpair2(add2(l[0], l[1]), lsum, t);
+            lsum += t;
         }
         const bool have = j1 > j0;
         if (ok && have && !__all_sync(0xffffffffu, mbar_wait(odone, 0))) {
@@ -796,8 +830,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         if (ok) {
             const int64_t prow = (int64_t)token * c.hq + head * c.rep + row % c.rep;
             const bool live = p >= 0;
-            const float inv = l > 0.f ? 1.0f / l : 0.f;
-            if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? l : 0.f);
+            const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+            if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? lsum : 0.f);
 #pragma unroll
             for (int w = 0; w < DB * 2; w++) {
                 uint32_t v[32];
@@ -820,11 +854,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                             uint32_t o[4];
 #pragma unroll
                             for (int i = 0; i < 4; i++)
-                                o[i] = pack_bf2(__uint_as_float(v[x + 2 * i]) * inv, __uint_as_float(v[x + 2 * i + 1]) * inv);
+                                o[i] = cvt_bf2(__uint_as_float(v[x + 2 * i]) * inv, __uint_as_float(v[x + 2 * i + 1]) * inv);
                             *reinterpret_cast<uint4 *>(dst + x) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
                 }
             }
+        }
         }
     }
     tc_fence_before();
@@ -863,7 +898,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const float inv = L > 0.f ? 1.0f / L : 0.f;
     if (d < c.D)
         *reinterpret_cast<uint2 *>(c.out + row / c.hq * c.out_stride + row % c.hq * c.D + d) =
-            make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+            make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
 }
 
 // the partial results' room in a workspace: 148 CTAs of 256 rows, whatever

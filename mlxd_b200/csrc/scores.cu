@@ -74,29 +74,6 @@ MLXD_DEV void sc_unpack(const uint4 &v, float (&x)[4]) {
 
 constexpr float SC_LOG2E = 1.4426950408889634f, SC_LN2 = 0.6931471805599453f;
 
-// two lanes of f32 in one instruction
-MLXD_DEV u64 pair2(float lo, float hi) {
-    u64 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-MLXD_DEV void unpair2(u64 v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-MLXD_DEV u64 add2(u64 a, u64 b) {
-    u64 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-MLXD_DEV u64 mul2(u64 a, u64 b) {
-    u64 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-MLXD_DEV u64 fma2(u64 a, u64 b, u64 c) {
-    u64 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // sums over what was seen but its largest logit: s of 2^z and w of z 2^z, z =
 // (x - ref) log2 e; best/at: the held-out logit (-inf: none above -inf yet)
 struct ScoreSums {
