@@ -16,6 +16,11 @@
 namespace mlxd {
 
 constexpr float LOG2E = 1.4426950408889634f;
+MLXD_DEV float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 struct AttnCall {
     const uint16_t *q;
@@ -119,6 +124,13 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(AttnCall c) {
             c.out[i * c.out_stride + (int64_t)h * c.D + lane * 8 + d] = f2bf(l > 0.f ? acc[d] / l : l);
 }
 
+// the partial results' room in a workspace: 148 CTAs of 256 rows, whatever
+// the call (more rows than that go unsplit, or in batches)
+constexpr int64_t AT_WS_ROWS = 148 * 256;
+static size_t at_ws_bytes(int D) { return (size_t)AT_WS_ROWS * ((D + 7) / 8 * 8 * 4 + 8) + 256; }
+
+static float2 *at_ws_ml(void *ws, int D) { return (float2 *)((char *)ws + (size_t)AT_WS_ROWS * D * 4); }
+
 // ---- few query rows per kv head (single tokens, tails): key-split warps
 //
 // Up to 16 query rows that share a kv head (the head group of one token, or of
@@ -135,21 +147,33 @@ __global__ void __launch_bounds__(128) attend_rows_kernel(AttnCall c) {
 // of a cluster merge at the end through (distributed) shared memory, in a
 // fixed order. Weights enter the value product as two bf16 terms (high and
 // low half), which costs idle tensor time and keeps them to 2^-17.
-constexpr int FR_MAXCL = 16;
+constexpr int FR_MAXCL = 8;                        // CTAs of a cluster (the portable size)
+constexpr int FR_PARTS = 56, FR_SRC = 64;          // splits of a prefix, and those with a cluster's CTAs
+
+struct FewCall {
+    int cluster;               // grid x is a cluster whose results meet, else each CTA's is partial
+    float *part_o;             // partial results [grid x][prow], or null: the whole result to out
+    float2 *part_ml;
+    int64_t prow;
+};
 
 template <int NU, int ROWS, int W>
-__global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constant__ AttnCall c) {
+__global__ void __launch_bounds__(W * 32)
+    attend_few_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ FewCall t) {
     constexpr int NW = (NU + 1) / 2, DP = NW * 64;
     extern __shared__ __align__(16) float fsm[];
     float *so = fsm;                               // [W][ROWS][DP]
     float *sm = so + W * ROWS * DP;                // [W][ROWS] maxima
     float *sl = sm + W * ROWS;                     // [W][ROWS] sums
+    float *sw = sl + W * ROWS;                     // [sources][ROWS] weights at the end
+    float *srow = sw + FR_SRC * ROWS;              // [ROWS]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
-    const int rank = blockIdx.x, ncta = gridDim.x;   // the cluster spans x
+    const int rank = blockIdx.x, ncta = gridDim.x;   // the item's CTAs
     const int head = blockIdx.y % c.hkv, tile = blockIdx.y / c.hkv, seq = blockIdx.z;
     const int rows_total = c.lens ? c.rep : c.n * c.rep, r0 = tile * ROWS, nrows = min(ROWS, rows_total - r0);
     auto token_of = [&](int r) { return c.lens ? seq : (r0 + r) / c.rep; };
     auto qhead_of = [&](int r) { return head * c.rep + (r0 + r) % c.rep; };
+    pdl_trigger();                                 // the join kernel may be put in place
     if (c.lens && c.lens[seq] < 0) return;         // a finished sequence: the whole cluster
 
     // the item's keys
@@ -277,7 +301,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
             const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
             if (__any_sync(0xffffffffu, mn > m)) {
-                const float a = exp2f((m - mu) * s2);
+                const float a = ex2((m - mu) * s2);
                 l *= a;
 #pragma unroll
                 for (int j = 0; j < NW * 8; j++) {
@@ -288,7 +312,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
             }
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const float e0 = exp2f((z[t][x] - mu) * s2), e1 = exp2f((z[t][x + 1] - mu) * s2);
+                const float e0 = ex2((z[t][x] - mu) * s2), e1 = ex2((z[t][x + 1] - mu) * s2);
                 l += e0 + e1;
                 const uint32_t h = cvt_bf2(e0, e1);
                 ph[2 * t + x / 2] = h;
@@ -346,7 +370,7 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
         if (M != -INFINITY)
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float a = exp2f((sm[w * ROWS + r] - M) * s2);
+                const float a = ex2((sm[w * ROWS + r] - M) * s2);
                 const float4 v = *reinterpret_cast<const float4 *>(so + (size_t)(w * ROWS + r) * DP + d);
                 acc.x = fmaf(a, v.x, acc.x);
                 acc.y = fmaf(a, v.y, acc.y);
@@ -360,98 +384,178 @@ __global__ void __launch_bounds__(W * 32) attend_few_kernel(const __grid_constan
         float M = -INFINITY, L = 0.f;
         for (int w = 0; w < W; w++) M = fmaxf(M, sm[w * ROWS + tid]);
         if (M != -INFINITY)
-            for (int w = 0; w < W; w++) L += sl[w * ROWS + tid] * exp2f((sm[w * ROWS + tid] - M) * s2);
+            for (int w = 0; w < W; w++) L += sl[w * ROWS + tid] * ex2((sm[w * ROWS + tid] - M) * s2);
         sm[tid] = M;
         sl[tid] = L;
     }
-    cluster_sync_all();
-    pdl_wait();                                    // the prefix half's results
-    // rows x features over the cluster's CTAs: ranks in order, then the prefix's splits
-    for (int i = rank * W * 32 + tid; i < nrows * (c.D / 4); i += ncta * W * 32) {
-        const int r = i / (c.D / 4), d = 4 * (i % (c.D / 4)), token = token_of(r), qh = qhead_of(r);
-        float M = -INFINITY;
-        for (int k = 0; k < ncta; k++) M = fmaxf(M, ld_cluster(sm + r, k));
-        const int64_t row = (int64_t)token * c.hq + qh, prow = (int64_t)c.n * c.hq;
-        for (int k = 0; k < c.parts; k++) M = fmaxf(M, c.part_ml[k * prow + row].x);
-        float L = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY) {
-            for (int k = 0; k < ncta; k++) {
-                const float a = exp2f((ld_cluster(sm + r, k) - M) * s2);
-                const float4 v = ld_cluster4(so + (size_t)r * DP + d, k);
-                L = fmaf(a, ld_cluster(sl + r, k), L);
-                acc.x = fmaf(a, v.x, acc.x);
-                acc.y = fmaf(a, v.y, acc.y);
-                acc.z = fmaf(a, v.z, acc.z);
-                acc.w = fmaf(a, v.w, acc.w);
+    const int ncl = t.cluster ? ncta : 1;            // CTAs whose results meet here
+    if (ncl > 1) cluster_sync_all();
+    else __syncthreads();
+    pdl_wait();                                      // the prefix half's results
+    // weights of the sources (cluster ranks in order, then the prefix's splits): a warp per row
+    const int64_t prow = (int64_t)c.n * c.hq;
+    const int nsrc = ncl + c.parts;
+    for (int r = warp; r < nrows; r += W) {
+        const int64_t row = (int64_t)token_of(r) * c.hq + qhead_of(r);
+        float mv[FR_SRC / 32], lv[FR_SRC / 32], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int u = 0; u < FR_SRC / 32; u++) {
+            const int k = 32 * u + lane;
+            mv[u] = -INFINITY;
+            lv[u] = 0.f;
+            if (k < ncl) {
+                mv[u] = ncl > 1 ? ld_cluster(sm + r, k) : sm[r];
+                lv[u] = ncl > 1 ? ld_cluster(sl + r, k) : sl[r];
+            } else if (k < nsrc) {
+                const float2 ml = c.part_ml[(k - ncl) * prow + row];
+                mv[u] = ml.x;
+                lv[u] = ml.y;
             }
-            for (int k = 0; k < c.parts; k++) {
-                const float2 ml = c.part_ml[k * prow + row];
-                const float a = exp2f((ml.x - M) * s2);
-                if (ml.x == -INFINITY) continue;
-                const float4 v = *reinterpret_cast<const float4 *>(c.part_o + (k * prow + row) * c.D + d);
-                L = fmaf(a, ml.y, L);
-                acc.x = fmaf(a, v.x, acc.x);
-                acc.y = fmaf(a, v.y, acc.y);
-                acc.z = fmaf(a, v.z, acc.z);
-                acc.w = fmaf(a, v.w, acc.w);
+            M = fmaxf(M, mv[u]);
+        }
+        M = warp_max(M);
+#pragma unroll
+        for (int u = 0; u < FR_SRC / 32; u++) {
+            const float a = mv[u] == -INFINITY ? 0.f : ex2((mv[u] - M) * s2);
+            L = fmaf(a, lv[u], L);
+            if (32 * u + lane < nsrc) sw[(32 * u + lane) * ROWS + r] = a;
+        }
+        L = warp_sum(L);
+        if (lane == 0) {
+            srow[r] = t.part_o ? 1.f : M == -INFINITY ? 0.f : 1.0f / L;   // a row that sees nothing is zero
+            if (t.part_o && rank % ncl == 0) t.part_ml[blockIdx.x / ncl * t.prow + row] = make_float2(M, L);
+        }
+    }
+    __syncthreads();
+    // rows x features over the CTAs that met
+    const int me = t.cluster ? rank : 0;
+    for (int i = me * W * 32 + tid; i < nrows * (c.D / 4); i += ncl * W * 32) {
+        const int r = i / (c.D / 4), d = 4 * (i % (c.D / 4)), token = token_of(r), qh = qhead_of(r);
+        const int64_t row = (int64_t)token * c.hq + qh;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](const float4 &v, int src) {
+            const float a = sw[src * ROWS + r];
+            acc.x = fmaf(a, v.x, acc.x);
+            acc.y = fmaf(a, v.y, acc.y);
+            acc.z = fmaf(a, v.z, acc.z);
+            acc.w = fmaf(a, v.w, acc.w);
+        };
+        const float *mine = so + (size_t)r * DP + d;
+        if (ncl == 1) {
+            add(*reinterpret_cast<const float4 *>(mine), 0);
+        } else {
+            for (int k = 0; k < ncl; k += 4) {       // four loads in flight
+                float4 v[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) v[u] = ld_cluster4(mine, min(k + u, ncl - 1));
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (k + u < ncl) add(v[u], k + u);
             }
         }
-        const float inv = M == -INFINITY ? 0.f : 1.0f / L;   // a row that sees nothing is zero
-        *reinterpret_cast<uint2 *>(c.out + token * c.out_stride + (int64_t)qh * c.D + d) =
-            make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
+        const float *po = c.part_o + row * c.D + d;
+        for (int k = 0; k < c.parts; k += 6) {
+            float4 v[6];
+#pragma unroll
+            for (int u = 0; u < 6; u++) {
+                // a split that saw nothing wrote no row
+                const bool live = k + u < c.parts && sw[(ncl + k + u) * ROWS + r] != 0.f;
+                v[u] = live ? *reinterpret_cast<const float4 *>(po + (k + u) * prow * c.D) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 6; u++)
+                if (k + u < c.parts) add(v[u], ncl + k + u);
+        }
+        if (t.part_o) {
+            *reinterpret_cast<float4 *>(t.part_o + (blockIdx.x / ncl * t.prow + row) * c.D + d) = acc;
+        } else {
+            const float inv = srow[r];
+            *reinterpret_cast<uint2 *>(c.out + token * c.out_stride + (int64_t)qh * c.D + d) =
+                make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
+        }
     }
-    cluster_sync_all();                            // no CTA leaves while its shared memory is read
+    if (ncl > 1) cluster_sync_all();                 // no CTA leaves while its shared memory is read
 }
 
 template <int NU, int ROWS, int W>
-static int launch_few(const AttnCall &c, int cl, int tiles, bool pdl, cudaStream_t st) {
+static int launch_few(const AttnCall &c, const FewCall &t, int splits, int tiles, bool pdl, cudaStream_t st) {
     constexpr int DP = (NU + 1) / 2 * 64;
     auto kern = attend_few_kernel<NU, ROWS, W>;
-    const size_t smem = (size_t)W * ROWS * (DP + 2) * 4;
-    if (!smem_allowed((const void *)kern, smem) || (cl > 8 && !nonportable_allowed((const void *)kern))) return -1;
+    const size_t smem = ((size_t)W * ROWS * (DP + 2) + (FR_SRC + 1) * ROWS) * 4;
+    if (!smem_allowed((const void *)kern, smem)) return -1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cl, c.hkv * tiles, c.lens ? c.n : 1);
+    cfg.gridDim = dim3(splits, c.hkv * tiles, c.lens ? c.n : 1);
     cfg.blockDim = dim3(W * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cl;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    int na = 0;
+    if (t.cluster) {
+        attr[na].id = cudaLaunchAttributeClusterDimension;
+        attr[na].val.clusterDim.x = splits;
+        attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+        na++;
+    }
+    if (pdl) {
+        attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[na].val.programmaticStreamSerializationAllowed = 1;
+        na++;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 2 : 1;
-    MLXD_CHECK(cudaLaunchKernelEx(&cfg, kern, c));
+    cfg.numAttrs = na;
+    MLXD_CHECK(cudaLaunchKernelEx(&cfg, kern, c, t));
     return 0;
 }
 
+template <int W>
+static int launch_few_w(const AttnCall &c, const FewCall &t, int rows, int splits, int tiles, bool pdl, cudaStream_t st) {
+    switch ((c.D + 31) / 32 * 2 + (rows > 8)) {
+    case 2: return launch_few<1, 8, W>(c, t, splits, tiles, pdl, st);
+    case 3: return launch_few<1, 16, W>(c, t, splits, tiles, pdl, st);
+    case 4: return launch_few<2, 8, W>(c, t, splits, tiles, pdl, st);
+    case 5: return launch_few<2, 16, W>(c, t, splits, tiles, pdl, st);
+    case 6: return launch_few<3, 8, W>(c, t, splits, tiles, pdl, st);
+    case 7: return launch_few<3, 16, W>(c, t, splits, tiles, pdl, st);
+    case 8: return launch_few<4, 8, W>(c, t, splits, tiles, pdl, st);
+    case 9: return launch_few<4, 16, W>(c, t, splits, tiles, pdl, st);
+    }
+    set_error("attention: head dim %d", c.D);
+    return -1;
+}
+
+static int launch_join(const AttnCall &c, cudaStream_t st);
+
 // rows: query rows of an item that share a kv head; keys: the most that an
-// item reads
-static int attend_few(const AttnCall &c, int rows, int keys, bool pdl, cudaStream_t st) {
+// item reads; ws: room for partial results (null: none are made)
+static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaStream_t st) {
     const int R = rows > 8 ? 16 : 8, tiles = (rows + R - 1) / R;
     if ((int64_t)c.hkv * tiles > 65535 || (c.lens && c.n > 65535)) {
         set_error("attention: too many rows for one launch");
         return -1;
     }
     const int64_t items = (int64_t)c.hkv * tiles * (c.lens ? c.n : 1);
-    // fill the SMs while every warp of 8 still has a step of 16 keys
-    int cl = 1;
-    while (cl < FR_MAXCL && items * cl * 2 <= num_sms() && keys > cl * 8 * 16) cl *= 2;
-    const int nu = (c.D + 31) / 32;
-    switch (nu * 2 + (R > 8)) {
-    case 2: return launch_few<1, 8, 8>(c, cl, tiles, pdl, st);
-    case 3: return launch_few<1, 16, 8>(c, cl, tiles, pdl, st);
-    case 4: return launch_few<2, 8, 8>(c, cl, tiles, pdl, st);
-    case 5: return launch_few<2, 16, 8>(c, cl, tiles, pdl, st);
-    case 6: return launch_few<3, 8, 8>(c, cl, tiles, pdl, st);
-    case 7: return launch_few<3, 16, 8>(c, cl, tiles, pdl, st);
-    case 8: return launch_few<4, 8, 8>(c, cl, tiles, pdl, st);
-    case 9: return launch_few<4, 16, 8>(c, cl, tiles, pdl, st);
+    FewCall t = {};
+    // CTAs per item: as many as fill the SMs while each of their 8 warps has two steps of 16 keys
+    int64_t s = num_sms() / items, most = (keys + 8 * 32 - 1) / (8 * 32);
+    if (s > most) s = most;
+    if (s > FR_PARTS) s = FR_PARTS;
+    if (s > AT_WS_ROWS / ((int64_t)c.n * c.hq)) s = AT_WS_ROWS / ((int64_t)c.n * c.hq);
+    if (s > 2 * FR_MAXCL && ws) {
+        // more than two clusters' worth: partial results and a second kernel
+        t.prow = (int64_t)c.n * c.hq;
+        t.part_o = (float *)ws;
+        t.part_ml = at_ws_ml(ws, c.D);
+        if (launch_few_w<8>(c, t, rows, (int)s, tiles, pdl, st)) return -1;
+        c.part_o = t.part_o;
+        c.part_ml = t.part_ml;
+        c.parts = (int)s;
+        return launch_join(c, st);
     }
-    set_error("attention: head dim %d", c.D);
-    return -1;
+    int cl = 1;
+    while (cl < FR_MAXCL && cl * 2 <= s) cl *= 2;
+    t.cluster = cl > 1;
+    // items enough for every SM: CTAs of 4 warps, two to an SM
+    return items >= num_sms() ? launch_few_w<4>(c, t, rows, cl, tiles, pdl, st) : launch_few_w<8>(c, t, rows, cl, tiles, pdl, st);
 }
 
 // ---- many query rows per kv head: tensor-core tiles
@@ -481,9 +585,6 @@ static int attend_few(const AttnCall &c, int rows, int keys, bool pdl, cudaStrea
 // Keys no row of the CTA sees may hold anything: their scores are masked and
 // their value rows zeroed in shared memory. Every wait is bounded; a launch
 // that gave up says so in a host word that the next call reports.
-#ifndef AT_POLY
-#define AT_POLY 0
-#endif
 constexpr int AT_THREADS = 384, AT_KT = 128, AT_ROWS = 256;
 
 template <int DB>
@@ -510,29 +611,6 @@ MLXD_DEV uint32_t span_bits(int s0, int lo, int hi) {
     const uint32_t up = h == 32 ? 0xffffffffu : (1u << h) - 1u;
     return l >= h ? 0u : up & (0xffffffffu << l);
 }
-MLXD_DEV float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// 2^x on the FMA pipe for two x <= 127: nearest integer n by adding 1.5 2^23,
-// a cubic for 2^(x - n) on [-1/2, 1/2] (relative error 7.5e-5, minimax fit;
-// the weights are rounded to 2^-9), n into the exponent. Below 2^-125: 2^-125.
-MLXD_DEV void ex2_pair(float &x0, float &x1) {
-    const uint64_t magic = pair2(12582912.f, 12582912.f), neg = pair2(-12582912.f, -12582912.f);
-    const uint64_t x = pair2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-    const uint64_t t = add2(x, magic);
-    const uint64_t n = add2(t, neg), f = fma2(n, pair2(-1.f, -1.f), x);
-    uint64_t p = fma2(f, pair2(5.517155e-2f, 5.517155e-2f), pair2(0.24261136f, 0.24261136f));
-    p = fma2(f, p, pair2(0.69326102f, 0.69326102f));
-    p = fma2(f, p, pair2(0.99992806f, 0.99992806f));
-    float p0, p1, t0, t1;
-    unpair2(p, p0, p1);
-    unpair2(t, t0, t1);
-    x0 = __uint_as_float(__float_as_uint(p0) + (__float_as_uint(t0) << 23));
-    x1 = __uint_as_float(__float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 template <int DB>
 __global__ void __launch_bounds__(AT_THREADS, 1)
     attend_tile_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
@@ -799,13 +877,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     const int w = 2 * h + x / 16, y = 2 * (x % 16);
                     float e0, e1;
                     unpair2(fma2(pair2(__uint_as_float(v[w][y]), __uint_as_float(v[w][y + 1])), ss, mm), e0, e1);
-                    if (AT_POLY && x % (AT_POLY + !AT_POLY) == AT_POLY - 1) {
-                        ex2_pair(e0, e1);
-                    } else {
-                        e0 = ex2(e0);
-                        e1 = ex2(e1);
-                    }
-                    pk[x] = cvt_bf2(e0, e1);
+                    pk[x] = cvt_bf2(ex2(e0), ex2(e1));
                     l[x & 1] = add2(l[x & 1], pair2(lo_bf(pk[x]), hi_bf(pk[x])));
                 }
                 tmem_st32(ts + 32 * h, pk);
@@ -877,22 +949,43 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     const int lane = threadIdx.x & 31;
     const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), prow = (int64_t)c.n * c.hq;
     if (row >= prow) return;
+    // lane k holds the weights of splits k and k + 32; the features are 4 a lane
     const float s2 = c.scale * LOG2E;
-    float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < c.parts; k++) M = fmaxf(M, c.part_ml[k * prow + row].x);
+    float w[2], M = -INFINITY, L = 0.f;
+    float2 ml[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const int k = 32 * u + lane;
+        ml[u] = k < c.parts ? c.part_ml[k * prow + row] : make_float2(-INFINITY, 0.f);
+        M = fmaxf(M, ml[u].x);
+    }
+    M = warp_max(M);
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        w[u] = ml[u].x == -INFINITY ? 0.f : ex2((ml[u].x - M) * s2);
+        L = fmaf(w[u], ml[u].y, L);
+    }
+    L = warp_sum(L);
     const int d = lane * 4;
+    const float *po = c.part_o + row * c.D + d;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < c.parts; k++) {
-        const float2 ml = c.part_ml[k * prow + row];
-        if (ml.x == -INFINITY) continue;
-        const float a = ex2((ml.x - M) * s2);
-        L = fmaf(a, ml.y, L);
-        if (d < c.D) {
-            const float4 v = *reinterpret_cast<const float4 *>(c.part_o + (k * prow + row) * c.D + d);
-            acc.x = fmaf(a, v.x, acc.x);
-            acc.y = fmaf(a, v.y, acc.y);
-            acc.z = fmaf(a, v.z, acc.z);
-            acc.w = fmaf(a, v.w, acc.w);
+    for (int k = 0; k < c.parts; k += 4) {
+        float4 v[4];
+        float a[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float lo = __shfl_sync(0xffffffffu, w[0], (k + u) & 31), hi = __shfl_sync(0xffffffffu, w[1], (k + u) & 31);
+            a[u] = k + u >= c.parts ? 0.f : k + u < 32 ? lo : hi;
+            // a split that saw nothing wrote no row
+            v[u] = d < c.D && a[u] != 0.f ? *reinterpret_cast<const float4 *>(po + (k + u) * prow * c.D)
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            acc.x = fmaf(a[u], v[u].x, acc.x);
+            acc.y = fmaf(a[u], v[u].y, acc.y);
+            acc.z = fmaf(a[u], v[u].z, acc.z);
+            acc.w = fmaf(a[u], v[u].w, acc.w);
         }
     }
     const float inv = L > 0.f ? 1.0f / L : 0.f;
@@ -901,10 +994,19 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
             make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
 }
 
-// the partial results' room in a workspace: 148 CTAs of 256 rows, whatever
-// the call (more rows than that go unsplit, or in batches)
-constexpr int64_t AT_WS_ROWS = 148 * AT_ROWS;
-static size_t at_ws_bytes(int D) { return (size_t)AT_WS_ROWS * ((D + 7) / 8 * 8 * 4 + 8) + 256; }
+static int launch_join(const AttnCall &c, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(((int64_t)c.n * c.hq + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    MLXD_CHECK(cudaLaunchKernelEx(&cfg, attend_join_kernel, c));
+    return 0;
+}
 
 template <int DB>
 static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &mk, const CUtensorMap &mv,
@@ -924,6 +1026,7 @@ static int tile_splits(const AttnCall &c, int keys) {
     int64_t s = num_sms() / pairs;
     if (s > (keys + AT_KT - 1) / AT_KT) s = (keys + AT_KT - 1) / AT_KT;
     if (s > AT_WS_ROWS / rows) s = AT_WS_ROWS / rows;
+    if (s > FR_PARTS) s = FR_PARTS;
     return s < 1 ? 1 : (int)s;
 }
 
@@ -995,7 +1098,7 @@ static int attend_tiles(AttnCall c, const mlxd_kv *kv, int layer, int splits, bo
     t.prow = (int64_t)c.n * c.hq;
     if (partial) {
         t.part_o = (float *)ws;
-        t.part_ml = (float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+        t.part_ml = at_ws_ml(ws, c.D);
     }
     t.fail = fail_word(false);
     return c.D <= 64 ? launch_tile<1>(c, t, kv->map_k, kv->map_v, st) : launch_tile<2>(c, t, kv->map_k, kv->map_v, st);
@@ -1016,7 +1119,7 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
     if (c.D > 128) return attend_rows(c, st);
     const int64_t span = (int64_t)c.window + c.n - 1 + c.sinks;
     const int keys = c.window && span < c.total ? (int)span : c.total;   // the most that one row group sees
-    if ((int64_t)c.n * c.rep <= 16 || c.n == 1) return attend_few(c, c.n * c.rep, keys, false, st);
+    if ((int64_t)c.n * c.rep <= 16 || c.n == 1) return attend_few(c, c.n * c.rep, keys, false, ws, st);
     if ((int64_t)c.n * c.rep > INT32_MAX - AT_ROWS || c.hkv > 65535) {
         set_error("kv_attend: too many query rows");
         return -1;
@@ -1025,11 +1128,9 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
     if (attend_tiles(c, kv, layer, splits, splits > 1, ws, st)) return -1;
     if (splits == 1) return 0;
     c.part_o = (const float *)ws;
-    c.part_ml = (const float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+    c.part_ml = at_ws_ml(ws, c.D);
     c.parts = splits;
-    attend_join_kernel<<<(unsigned)(((int64_t)c.n * c.hq + 7) / 8), 256, 0, st>>>(c);
-    MLXD_CHECK(cudaGetLastError());
-    return 0;
+    return launch_join(c, st);
 }
 
 // sequences in batches whose partial rows fit the workspace: the prefix on
@@ -1055,10 +1156,10 @@ static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
             const int splits = tile_splits(b, c.prefix);
             if (attend_tiles(b, kv, layer, splits, true, ws, st)) return -1;
             b.part_o = (const float *)ws;
-            b.part_ml = (const float2 *)((char *)ws + (size_t)AT_WS_ROWS * c.D * 4);
+            b.part_ml = at_ws_ml(ws, c.D);
             b.parts = splits;
         }
-        if (attend_few(b, b.rep, c.tcap, c.prefix > 0, st)) return -1;
+        if (attend_few(b, b.rep, c.tcap, c.prefix > 0, nullptr, st)) return -1;
     }
     return 0;
 }
