@@ -134,19 +134,25 @@ static float2 *at_ws_ml(void *ws, int D) { return (float2 *)((char *)ws + (size_
 // ---- few query rows per kv head (single tokens, tails): key-split warps
 //
 // Up to 16 query rows that share a kv head (the head group of one token, or of
-// a few) against 16 keys a step, on mma.m16n8k16. Bound by HBM: the arithmetic
-// is 8 heads deep at most, so the tensor cores only keep it off the FMA pipe;
-// every key row is read once, straight into registers in fragment order:
-//   scores   the contraction runs over features, whose order is free: lane
-//            (g, c) = (lane / 4, lane % 4) holds the 16 bytes of features
-//            32 u + 8 c of key g, which are the B fragments of two k-steps;
-//   values   lane (g, c) holds features 64 w + 8 g .. + 7 of keys 2c, 2c + 1,
-//            2c + 8, 2c + 9; the column order is free too, so the pairs of one
-//            feature of two keys are one byte permute away from B fragments.
+// a few) against 16 keys a step, on mma.m16n8k16 with the keys and then the
+// features as its 16 rows and the query rows as its 8 columns (the other way
+// round takes twice the MMAs, which at 28 clocks each are the limit here, not
+// HBM: 41 us instead of 29 at one token over 32768 positions). Every key row is
+// read once, in fragment order:
+//   scores   S^T = K Q^T: the contraction runs over features, whose order is
+//            free: lane (g, c) = (lane / 4, lane % 4) holds the 16 bytes of
+//            features 32 u + 8 c of keys g and g + 8, the A fragments of two
+//            k-steps;
+//   values   O^T = V^T P^T: lane (g, c) holds features 64 w + 8 g .. + 7 of keys
+//            2c, 2c + 1, 2c + 8, 2c + 9; the row order is free too, so the
+//            pairs of one feature of two keys are one byte permute away from A
+//            fragments; P^T is a transposing move of the weights.
 // A warp owns a run of steps with its own running maximum; warps and the CTAs
 // of a cluster merge at the end through (distributed) shared memory, in a
-// fixed order. Weights enter the value product as two bf16 terms (high and
-// low half), which costs idle tensor time and keeps them to 2^-17.
+// fixed order. Weights enter the value product as two bf16 terms (to 2^-17):
+// with up to 4 rows the low terms fill the other 4 columns, with up to 8 they
+// take a second MMA; with 16 rows that would cost what HBM leaves, so there the
+// weights are rounded to bf16 and the row sum adds the rounded ones.
 constexpr int FR_MAXCL = 8;                        // CTAs of a cluster (the portable size)
 constexpr int FR_PARTS = 56, FR_SRC = 64;          // splits of a prefix, and those with a cluster's CTAs
 
@@ -157,13 +163,26 @@ struct FewCall {
     int64_t prow;
 };
 
+// shared memory of a warp: its ring, later its results
+constexpr int FR_DEPTH = 3;
+__host__ __device__ constexpr int fr_warp_floats(int nu, int rows) {
+    const int nw = (nu + 1) / 2, ring = FR_DEPTH * (2 * nu + 4 * nw) * 32 * 4, res = rows * nw * 64;
+    return ring > res ? ring : res;
+}
+MLXD_DEV uint32_t transpose8(uint32_t v) {           // 8 x 8 bf16 across the warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 template <int NU, int ROWS, int W>
 __global__ void __launch_bounds__(W * 32)
     attend_few_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ FewCall t) {
-    constexpr int NW = (NU + 1) / 2, DP = NW * 64;
+    constexpr int NW = (NU + 1) / 2, DP = NW * 64, NT = ROWS > 8 ? 2 : 1;
+    constexpr bool LOW = ROWS <= 8;                  // the weights' low terms too
     extern __shared__ __align__(16) float fsm[];
-    float *so = fsm;                               // [W][ROWS][DP]
-    float *sm = so + W * ROWS * DP;                // [W][ROWS] maxima
+    float *so = fsm;                               // [W][ROWS][DP], in the rings' place
+    float *sm = so + W * fr_warp_floats(NU, ROWS);   // [W][ROWS] maxima
     float *sl = sm + W * ROWS;                     // [W][ROWS] sums
     float *sw = sl + W * ROWS;                     // [sources][ROWS] weights at the end
     float *srow = sw + FR_SRC * ROWS;              // [ROWS]
@@ -172,7 +191,7 @@ __global__ void __launch_bounds__(W * 32)
     const int head = blockIdx.y % c.hkv, tile = blockIdx.y / c.hkv, seq = blockIdx.z;
     const int rows_total = c.lens ? c.rep : c.n * c.rep, r0 = tile * ROWS, nrows = min(ROWS, rows_total - r0);
     auto token_of = [&](int r) { return c.lens ? seq : (r0 + r) / c.rep; };
-    auto qhead_of = [&](int r) { return head * c.rep + (r0 + r) % c.rep; };
+    auto qhead_of = [&](int r) { return head * c.rep + (c.lens || c.n == 1 ? r0 + r : (r0 + r) % c.rep); };
     pdl_trigger();                                 // the join kernel may be put in place
     if (c.lens && c.lens[seq] < 0) return;         // a finished sequence: the whole cluster
 
@@ -198,167 +217,205 @@ __global__ void __launch_bounds__(W * 32)
     const int ns = na + nc + nb, wg = rank * W + warp, nwg = ncta * W;
     const int st0 = (int)((int64_t)ns * wg / nwg), st1 = (int)((int64_t)ns * (wg + 1) / nwg);
 
-    // query fragments: rows g and g + 8, features in the keys' order
-    uint32_t qa[NU][ROWS > 8 ? 8 : 4];
+    // query fragments: column g (of each column tile), features in the keys' order
+    uint4 qb[NT][NU];
 #pragma unroll
-    for (int u = 0; u < NU; u++)
+    for (int i = 0; i < NT; i++) {
+        const int r = ROWS == 4 ? g & 3 : g + 8 * i;
+        const uint16_t *q = c.q + token_of(r) * c.q_stride + (int64_t)qhead_of(r) * c.D + 8 * cc;
 #pragma unroll
-        for (int hf = 0; hf < (ROWS > 8 ? 2 : 1); hf++) {
-            const int r = g + 8 * hf, f = 32 * u + 8 * cc;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < nrows && f < c.D)
-                v = *reinterpret_cast<const uint4 *>(c.q + token_of(r) * c.q_stride + (int64_t)qhead_of(r) * c.D + f);
-            qa[u][4 * hf] = v.x;
-            qa[u][4 * hf + 1] = v.y;
-            qa[u][4 * hf + 2] = v.z;
-            qa[u][4 * hf + 3] = v.w;
-        }
+        for (int u = 0; u < NU; u++)
+            qb[i][u] = r < nrows && 32 * u + 8 * cc < c.D ? ldg_nc_v4(q + 32 * u) : make_uint4(0, 0, 0, 0);
+    }
+    // this lane's columns 2 cc and 2 cc + 1 of a column tile: rows, positions, statistics
+    auto row_of = [&](int i, int x) { return ROWS == 4 ? (2 * cc + x) & 3 : 8 * i + 2 * cc + x; };
     const bool multi = pmin != pmax;               // rows at several positions: masks per row
-    const int p0 = multi && g < nrows ? query_pos(c, token_of(g)) : pmax;
-    const int p1 = multi && g + 8 < nrows ? query_pos(c, token_of(g + 8)) : pmax;
+    int p[NT][2];
+    float m[NT][2], l[NT][2], o[NT][NW * 4][4];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            p[i][x] = multi && row_of(i, x) < nrows ? query_pos(c, token_of(row_of(i, x))) : pmax;
+            m[i][x] = -INFINITY;
+            l[i][x] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NW * 4; j++) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    }
     const float s2 = c.scale * LOG2E;
 
-    float o[NW * 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-#pragma unroll
-    for (int j = 0; j < NW * 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-
     auto step_slots = [&](int st, int &s, int &e) {
-        if (st < na) {
-            s = 16 * st;
-            e = sp.a1;
-        } else if (st < na + nc) {
-            s = sp.c0 + 16 * (st - na);
-            e = sp.c1;
-        } else {
-            s = sp.b0 + 16 * (st - na - nc);
-            e = sp.b1;
-        }
+        const bool a = st < na, b = st >= na + nc;
+        s = a ? 16 * st : b ? sp.b0 + 16 * (st - na - nc) : sp.c0 + 16 * (st - na);
+        e = a ? sp.a1 : b ? sp.b1 : sp.c1;
     };
-    uint4 kr[NU][2], vr[NW][4];
-    auto load_k = [&](int st) {
-        int s, e;
-        step_slots(st, s, e);
+    // A step's rows go through a ring of FR_DEPTH stages in shared memory in which every lane reads back what
+    // it copied itself: deep prefetch without registers, layouts or barriers.
+    constexpr int KV = 2 * NU + 4 * NW;              // 16-byte pieces of a lane per step
+    uint4 *ring = reinterpret_cast<uint4 *>(fsm) + (size_t)warp * FR_DEPTH * KV * 32 + lane;
+    int put = 0, get = 0;                            // ring stages
+#pragma unroll 1
+    for (int st = st0 - (FR_DEPTH - 1); st < st1; st++) {
+        const int ahead = st + FR_DEPTH - 1;
+        if (ahead < st1) {
+            int s, e;
+            step_slots(ahead, s, e);
+            uint4 *dst = ring + put * KV * 32;
+            put = put + 1 == FR_DEPTH ? 0 : put + 1;
+            // past the end: the last row again, its score masked; past D: zeros
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            // past the end: the last row again, its score masked
-            const uint16_t *row = kb + (size_t)min(s + 8 * t + g, e - 1) * c.D + 8 * cc;
+            for (int i = 0; i < 2; i++) {
+                const uint16_t *row = kb + (size_t)min(s + 8 * i + g, e - 1) * c.D + 8 * cc;
 #pragma unroll
-            for (int u = 0; u < NU; u++) kr[u][t] = 32 * u + 8 * cc < c.D ? ldg_nc_v4(row + 32 * u) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    auto load_v = [&](int st) {
-        int s, e;
-        step_slots(st, s, e);
+                for (int u = 0; u < NU; u++) {
+                    const bool in = 32 * u + 8 * cc < c.D;
+                    cp_async16_zfill(dst + (2 * u + i) * 32, in ? row + 32 * u : kb, in);
+                }
+            }
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const uint16_t *row = vb + (size_t)min(s + 2 * cc + (t & 1) + 8 * (t >> 1), e - 1) * c.D + 8 * g;
+            for (int i = 0; i < 4; i++) {
+                const uint16_t *row = vb + (size_t)min(s + 2 * cc + (i & 1) + 8 * (i >> 1), e - 1) * c.D + 8 * g;
 #pragma unroll
-            for (int w = 0; w < NW; w++) vr[w][t] = 64 * w + 8 * g < c.D ? ldg_nc_v4(row + 64 * w) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    if (st0 < st1) {
-        load_k(st0);
-        load_v(st0);
-    }
-    for (int st = st0; st < st1; st++) {
-        float z[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            z[t][0] = z[t][1] = z[t][2] = z[t][3] = 0.f;
-#pragma unroll
-            for (int u = 0; u < NU; u++) {
-                uint32_t a0[4] = {qa[u][0], ROWS > 8 ? qa[u][ROWS > 8 ? 4 : 0] : 0u, qa[u][1],
-                                  ROWS > 8 ? qa[u][ROWS > 8 ? 5 : 0] : 0u};
-                uint32_t a1[4] = {qa[u][2], ROWS > 8 ? qa[u][ROWS > 8 ? 6 : 0] : 0u, qa[u][3],
-                                  ROWS > 8 ? qa[u][ROWS > 8 ? 7 : 0] : 0u};
-                mma_bf16_16816(z[t], a0, kr[u][t].x, kr[u][t].y);
-                mma_bf16_16816(z[t], a1, kr[u][t].z, kr[u][t].w);
+                for (int w = 0; w < NW; w++) {
+                    const bool in = 64 * w + 8 * g < c.D;
+                    cp_async16_zfill(dst + (2 * NU + 4 * w + i) * 32, in ? row + 64 * w : vb, in);
+                }
             }
         }
-        if (st + 1 < st1) load_k(st + 1);
+        cp_async_commit();
+        if (st < st0) continue;                      // the ring's first stages
+        cp_async_wait<FR_DEPTH - 1>();
+        const uint4 *src = ring + get * KV * 32;
+        get = get + 1 == FR_DEPTH ? 0 : get + 1;
+        // scores of keys g and g + 8 (rows) in this lane's columns, as two chains
+        float z[NT][4], z1[NT][4];
+#pragma unroll
+        for (int i = 0; i < NT; i++)
+#pragma unroll
+            for (int x = 0; x < 4; x++) z[i][x] = z1[i][x] = 0.f;
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            const uint4 k0 = src[2 * u * 32], k1 = src[(2 * u + 1) * 32];
+            const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
+#pragma unroll
+            for (int i = 0; i < NT; i++) {
+                mma_bf16_16816(z[i], a0, qb[i][u].x, qb[i][u].y);
+                mma_bf16_16816(z1[i], a1, qb[i][u].z, qb[i][u].w);
+            }
+        }
         int s, e;
         step_slots(st, s, e);
-        if (s + 16 > e || multi) {
+        const bool edge = s + 16 > e || multi;
+        uint32_t ph[NT][2], pl[NT][2];               // weights as B fragments
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+        for (int i = 0; i < NT; i++) {
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int key = s + 8 * t + 2 * cc + x;
-                    bool see0 = key < e, see1 = see0;
+            for (int x = 0; x < 4; x++) z[i][x] += z1[i][x];
+            if (edge)
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const int key = s + g + 8 * (x >> 1), pr = p[i][x & 1];
+                    bool see = key < e;
                     if (multi) {
                         const int kp = slot_pos(c, key);
-                        see0 = see0 && kp <= p0 && (kp >= window_lo(c, p0) || kp < c.sinks);
-                        see1 = see1 && kp <= p1 && (kp >= window_lo(c, p1) || kp < c.sinks);
+                        see = see && kp <= pr && (kp >= window_lo(c, pr) || kp < c.sinks);
                     }
-                    if (!see0) z[t][x] = -INFINITY;
-                    if (!see1) z[t][2 + x] = -INFINITY;
+                    if (!see) z[i][x] = -INFINITY;
                 }
+            float mu[2];
+            bool grow = false;
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                float mx = fmaxf(z[i][x], z[i][2 + x]);
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                mu[x] = fmaxf(m[i][x], mx);
+                grow = grow || mu[x] > m[i][x];
+            }
+            if (__any_sync(0xffffffffu, grow))
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const float a = mu[x] == -INFINITY ? 1.f : ex2((m[i][x] - mu[x]) * s2);
+                    m[i][x] = mu[x];
+                    l[i][x] *= a;
+#pragma unroll
+                    for (int j = 0; j < NW * 4; j++) {
+                        o[i][j][x] *= a;
+                        o[i][j][2 + x] *= a;
+                    }
+                }
+            float w[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) w[x] = ex2((z[i][x] - (mu[x & 1] == -INFINITY ? 0.f : mu[x & 1])) * s2);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {            // key g, key g + 8
+                const uint32_t hi = cvt_bf2(w[2 * k], w[2 * k + 1]);
+                if constexpr (LOW) {
+                    const uint32_t lo = cvt_bf2(w[2 * k] - lo_bf(hi), w[2 * k + 1] - hi_bf(hi));
+                    l[i][0] += w[2 * k];
+                    l[i][1] += w[2 * k + 1];
+                    ph[i][k] = transpose8(ROWS == 4 && cc >= 2 ? lo : hi);
+                    if (ROWS == 8) pl[i][k] = transpose8(lo);
+                } else {
+                    l[i][0] += lo_bf(hi);
+                    l[i][1] += hi_bf(hi);
+                    ph[i][k] = transpose8(hi);
+                }
+            }
         }
-        uint32_t ph[4], pl[4];
-        auto half = [&](int x, float &m, float &l) {
-            float mx = fmaxf(fmaxf(z[0][x], z[0][x + 1]), fmaxf(z[1][x], z[1][x + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn;
-            if (__any_sync(0xffffffffu, mn > m)) {
-                const float a = ex2((m - mu) * s2);
-                l *= a;
-#pragma unroll
-                for (int j = 0; j < NW * 8; j++) {
-                    o[j][x] *= a;
-                    o[j][x + 1] *= a;
-                }
-                m = mn;
-            }
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const float e0 = ex2((z[t][x] - mu) * s2), e1 = ex2((z[t][x + 1] - mu) * s2);
-                l += e0 + e1;
-                const uint32_t h = cvt_bf2(e0, e1);
-                ph[2 * t + x / 2] = h;
-                pl[2 * t + x / 2] = cvt_bf2(e0 - lo_bf(h), e1 - hi_bf(h));
-            }
-        };
-        half(0, m0, l0);
-        if constexpr (ROWS > 8) half(2, m1, l1);
-        else ph[1] = ph[3] = pl[1] = pl[3] = 0u;
 #pragma unroll
         for (int w = 0; w < NW; w++) {
-            const uint32_t *y0 = &vr[w][0].x, *y1 = &vr[w][1].x, *y2 = &vr[w][2].x, *y3 = &vr[w][3].x;
+            uint4 v[4];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-                const uint32_t b0 = __byte_perm(y0[j / 2], y1[j / 2], sel), b1 = __byte_perm(y2[j / 2], y3[j / 2], sel);
-                mma_bf16_16816(o[8 * w + j], ph, b0, b1);
-                mma_bf16_16816(o[8 * w + j], pl, b0, b1);
+            for (int i = 0; i < 4; i++) v[i] = src[(2 * NU + 4 * w + i) * 32];
+            const uint32_t *y0 = &v[0].x, *y1 = &v[1].x, *y2 = &v[2].x, *y3 = &v[3].x;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {            // features 2 j (rows g) and 2 j + 1 (rows g + 8)
+                const uint32_t a[4] = {__byte_perm(y0[j], y1[j], 0x5410), __byte_perm(y0[j], y1[j], 0x7632),
+                                       __byte_perm(y2[j], y3[j], 0x5410), __byte_perm(y2[j], y3[j], 0x7632)};
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    mma_bf16_16816(o[i][4 * w + j], a, ph[i][0], ph[i][1]);
+                    if (ROWS == 8) mma_bf16_16816(o[i][4 * w + j], a, pl[i][0], pl[i][1]);
+                }
             }
         }
-        if (st + 1 < st1) load_v(st + 1);
     }
+    cp_async_wait<0>();
+    __syncthreads();                                 // the rings become the warps' results
 
-    // row sums over the quad, then this warp's result to shared memory
 #pragma unroll
-    for (int hf = 0; hf < (ROWS > 8 ? 2 : 1); hf++) {
-        float l = hf ? l1 : l0;
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        const int r = g + 8 * hf;
-        if (cc == 0) {
-            sm[warp * ROWS + r] = hf ? m1 : m0;
-            sl[warp * ROWS + r] = l;
+    for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            // the column's sum over its 8 lanes, then this warp's result to shared memory
+            float sum = l[i][x];
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            const int r = row_of(i, x);
+            if (g == 0 && (ROWS > 4 || cc < 2)) {
+                sm[warp * ROWS + r] = m[i][x];
+                sl[warp * ROWS + r] = sum;
+            }
+            float *dst = so + (size_t)(warp * ROWS + r) * DP + 8 * g;
+#pragma unroll
+            for (int w = 0; w < NW; w++) {
+                float f[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    f[2 * j] = o[i][4 * w + j][x];
+                    f[2 * j + 1] = o[i][4 * w + j][2 + x];
+                }
+                if (ROWS == 4)                       // the low terms' columns
+#pragma unroll
+                    for (int j = 0; j < 8; j++) f[j] += __shfl_xor_sync(0xffffffffu, f[j], 2);
+                if (ROWS > 4 || cc < 2) {
+                    *reinterpret_cast<float4 *>(dst + 64 * w) = make_float4(f[0], f[1], f[2], f[3]);
+                    *reinterpret_cast<float4 *>(dst + 64 * w + 4) = make_float4(f[4], f[5], f[6], f[7]);
+                }
+            }
         }
-        // columns 2 cc and 2 cc + 1 of tile j are features 64 w + 16 cc + j and + 8 + j
-        float *dst = so + (size_t)(warp * ROWS + r) * DP;
-#pragma unroll
-        for (int w = 0; w < NW; w++)
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int j = 0; j < 8; j += 4)
-                    *reinterpret_cast<float4 *>(dst + 64 * w + 16 * cc + 8 * x + j) =
-                        make_float4(o[8 * w + j][2 * hf + x], o[8 * w + j + 1][2 * hf + x],
-                                    o[8 * w + j + 2][2 * hf + x], o[8 * w + j + 3][2 * hf + x]);
-    }
     __syncthreads();
     // the CTA's warps into warp 0's rows
     for (int i = tid; i < nrows * (DP / 4); i += W * 32) {
@@ -479,9 +536,8 @@ __global__ void __launch_bounds__(W * 32)
 
 template <int NU, int ROWS, int W>
 static int launch_few(const AttnCall &c, const FewCall &t, int splits, int tiles, bool pdl, cudaStream_t st) {
-    constexpr int DP = (NU + 1) / 2 * 64;
     auto kern = attend_few_kernel<NU, ROWS, W>;
-    const size_t smem = ((size_t)W * ROWS * (DP + 2) + (FR_SRC + 1) * ROWS) * 4;
+    const size_t smem = ((size_t)W * (fr_warp_floats(NU, ROWS) + 2 * ROWS) + (FR_SRC + 1) * ROWS) * 4;
     if (!smem_allowed((const void *)kern, smem)) return -1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, c.hkv * tiles, c.lens ? c.n : 1);
@@ -507,17 +563,19 @@ static int launch_few(const AttnCall &c, const FewCall &t, int splits, int tiles
     return 0;
 }
 
+template <int NU, int W>
+static int launch_few_rows(const AttnCall &c, const FewCall &t, int R, int splits, int tiles, bool pdl, cudaStream_t st) {
+    return R == 4   ? launch_few<NU, 4, W>(c, t, splits, tiles, pdl, st)
+           : R == 8 ? launch_few<NU, 8, W>(c, t, splits, tiles, pdl, st)
+                    : launch_few<NU, 16, W>(c, t, splits, tiles, pdl, st);
+}
 template <int W>
-static int launch_few_w(const AttnCall &c, const FewCall &t, int rows, int splits, int tiles, bool pdl, cudaStream_t st) {
-    switch ((c.D + 31) / 32 * 2 + (rows > 8)) {
-    case 2: return launch_few<1, 8, W>(c, t, splits, tiles, pdl, st);
-    case 3: return launch_few<1, 16, W>(c, t, splits, tiles, pdl, st);
-    case 4: return launch_few<2, 8, W>(c, t, splits, tiles, pdl, st);
-    case 5: return launch_few<2, 16, W>(c, t, splits, tiles, pdl, st);
-    case 6: return launch_few<3, 8, W>(c, t, splits, tiles, pdl, st);
-    case 7: return launch_few<3, 16, W>(c, t, splits, tiles, pdl, st);
-    case 8: return launch_few<4, 8, W>(c, t, splits, tiles, pdl, st);
-    case 9: return launch_few<4, 16, W>(c, t, splits, tiles, pdl, st);
+static int launch_few_w(const AttnCall &c, const FewCall &t, int R, int splits, int tiles, bool pdl, cudaStream_t st) {
+    switch ((c.D + 31) / 32) {
+    case 1: return launch_few_rows<1, W>(c, t, R, splits, tiles, pdl, st);
+    case 2: return launch_few_rows<2, W>(c, t, R, splits, tiles, pdl, st);
+    case 3: return launch_few_rows<3, W>(c, t, R, splits, tiles, pdl, st);
+    case 4: return launch_few_rows<4, W>(c, t, R, splits, tiles, pdl, st);
     }
     set_error("attention: head dim %d", c.D);
     return -1;
@@ -528,7 +586,7 @@ static int launch_join(const AttnCall &c, cudaStream_t st);
 // rows: query rows of an item that share a kv head; keys: the most that an
 // item reads; ws: room for partial results (null: none are made)
 static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaStream_t st) {
-    const int R = rows > 8 ? 16 : 8, tiles = (rows + R - 1) / R;
+    const int R = rows > 8 ? 16 : rows > 4 ? 8 : 4, tiles = (rows + R - 1) / R;
     if ((int64_t)c.hkv * tiles > 65535 || (c.lens && c.n > 65535)) {
         set_error("attention: too many rows for one launch");
         return -1;
@@ -545,7 +603,7 @@ static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaSt
         t.prow = (int64_t)c.n * c.hq;
         t.part_o = (float *)ws;
         t.part_ml = at_ws_ml(ws, c.D);
-        if (launch_few_w<8>(c, t, rows, (int)s, tiles, pdl, st)) return -1;
+        if (launch_few_w<8>(c, t, R, (int)s, tiles, pdl, st)) return -1;
         c.part_o = t.part_o;
         c.part_ml = t.part_ml;
         c.parts = (int)s;
@@ -555,7 +613,7 @@ static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaSt
     while (cl < FR_MAXCL && cl * 2 <= s) cl *= 2;
     t.cluster = cl > 1;
     // items enough for every SM: CTAs of 4 warps, two to an SM
-    return items >= num_sms() ? launch_few_w<4>(c, t, rows, cl, tiles, pdl, st) : launch_few_w<8>(c, t, rows, cl, tiles, pdl, st);
+    return items >= num_sms() ? launch_few_w<4>(c, t, R, cl, tiles, pdl, st) : launch_few_w<8>(c, t, R, cl, tiles, pdl, st);
 }
 
 // ---- many query rows per kv head: tensor-core tiles
