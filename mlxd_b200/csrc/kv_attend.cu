@@ -636,7 +636,6 @@ static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaSt
 //                      relative to the maximum in use, so any will do).
 //
 // While one query tile is in its softmax the tensor cores work on the other.
-// The row sum adds the rounded weights, so that sum and numerator weigh alike.
 // Bound by the exponentials (128 x 128 per tile at 16 a clock and SM, 1024
 // clocks) and the tensor cores (2 x 512 clocks) alike when rows are many, by
 // HBM when a prefix is long and the rows are few.
@@ -669,7 +668,8 @@ MLXD_DEV uint32_t span_bits(int s0, int lo, int hi) {
     const uint32_t up = h == 32 ? 0xffffffffu : (1u << h) - 1u;
     return l >= h ? 0u : up & (0xffffffffu << l);
 }
-template <int DB>
+// BK: a CTA takes 128 rows, its two softmax halves alternating key tiles
+template <int DB, bool BK>
 __global__ void __launch_bounds__(AT_THREADS, 1)
     attend_tile_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                        const __grid_constant__ AttnCall c, const __grid_constant__ TileCall t) {
@@ -679,14 +679,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     unsigned char *sm = reinterpret_cast<unsigned char *>(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *kfull = reinterpret_cast<uint64_t *>(sm + L::BARS);
     uint64_t *kempty = kfull + NS, *vfull = kempty + NS, *vempty = vfull + NS;
-    uint64_t *sfull = vempty + NS, *pfull = sfull + 2, *odone = pfull + 4;   // pfull[2 t + half]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(odone + 1);
-    __shared__ int s_pmin, s_pmax, s_fail;
+    uint64_t *sfull = vempty + NS, *pfull = sfull + 2, *qfull = pfull + 4, *odone = qfull + 1, *xdone = odone + 1;   // pfull[2 t + half]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(xdone + 1);
+    __shared__ int s_min[8], s_max[8], s_fail;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int head = blockIdx.y, rows = c.n * c.rep;
-    const int r0 = (gridDim.x - 1 - blockIdx.x) * AT_ROWS;   // the longest rows first
-    const int nq = rows - r0 > 128 ? 2 : 1;
+    const int r0 = (gridDim.x - 1 - blockIdx.x) * (BK ? 128 : AT_ROWS);   // the longest rows first
+    const int nq = BK || rows - r0 > 128 ? 2 : 1;
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
             mbar_init(&kfull[i], 1);
@@ -696,9 +696,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         for (int i = 0; i < 2; i++) mbar_init(&sfull[i], 1);
         for (int i = 0; i < 4; i++) mbar_init(&pfull[i], 4);
+        mbar_init(qfull, 8);
         mbar_init(odone, 1);
-        s_pmin = INT32_MAX;
-        s_pmax = -1;
+        mbar_init(xdone, 4);
         s_fail = 0;
         fence_mbar_init();
     }
@@ -707,34 +707,27 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                      "r"(512));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    if (warp >= 4) {                                 // positions of the CTA's 256 rows
+        const int i = tid - 128, r = r0 + (BK ? i & 127 : i), p = r < rows ? query_pos(c, r / c.rep) : -1;
+        const int lo = __reduce_min_sync(0xffffffffu, p < 0 ? INT32_MAX : p), hi = __reduce_max_sync(0xffffffffu, p);
+        if (lane == 0) {
+            s_min[warp - 4] = lo;
+            s_max[warp - 4] = hi;
+        }
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_trigger();   // every CTA is on an SM: the tails may start on free ones
-    // positions of the CTA's rows, and the query tiles (zero past the rows and D)
-    if (tid < AT_ROWS && r0 + tid < rows) {
-        const int p = query_pos(c, (r0 + tid) / c.rep);
-        if (p >= 0) {
-            atomicMin(&s_pmin, p);
-            atomicMax(&s_pmax, p);
-        }
+    int pmin = s_min[0], pmax = s_max[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        pmin = min(pmin, s_min[i]);
+        pmax = max(pmax, s_max[i]);
     }
-    for (int i = tid; i < nq * 128 * DB * 8; i += AT_THREADS) {
-        const int r = i / (DB * 8), ch = i % (DB * 8);   // 16-byte chunk of the row
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r0 + r < rows && ch * 8 < c.D) {
-            const int token = (r0 + r) / c.rep, qh = head * c.rep + (r0 + r) % c.rep;
-            v = ldg_nc_v4(c.q + token * c.q_stride + (int64_t)qh * c.D + ch * 8);
-        }
-        *reinterpret_cast<uint4 *>(sm + L::Q + (r >> 7) * L::TILE + (ch >> 3) * L::BLOCK + (r & 127) * 128 +
-                                   (((ch & 7) ^ (r & 7)) << 4)) = v;
-    }
-    fence_proxy_async();
-    __syncthreads();
 
     // the visible slots as tiles: sinks, a ring's wrapped end, the rest
-    const int pmin = s_pmin, pmax = s_pmax;
     int a1 = 0, c0 = 0, c1 = 0, b0 = 0, b1 = 0;      // tile ranges [0, a1), [c0, c1), [b0, b1)
     Span all = {0, 0, 0, 0, 0};                      // the slots any row sees
     if (pmax >= 0) {
@@ -751,6 +744,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
     const int nt = a1 + (c1 - c0) + (b1 - b0);
     const int j0 = (int)((int64_t)nt * blockIdx.z / t.splits), j1 = (int)((int64_t)nt * (blockIdx.z + 1) / t.splits);
+    // key tile n of query tile i, counted from j0
+    auto key_tile = [&](int i, int n) { return BK ? 2 * n + i : n; };
     auto tile_slot = [&](int j) {
         const int k = j < a1 ? j : j < a1 + c1 - c0 ? c0 + j - a1 : b0 + j - a1 - (c1 - c0);
         return k * AT_KT;
@@ -792,7 +787,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             const uint64_t qd = umma_desc_sw128(smem_u32(sm + L::Q)), kd = umma_desc_sw128(smem_u32(sm + L::K));
             const uint64_t vd = umma_desc_sw128_mn(smem_u32(sm + L::V), L::BLOCK);
             auto qk = [&](int i, int n) {            // S_i = Q_i K_n^T
-                const uint64_t qt = qd + i * (L::TILE >> 4), kt = kd + (n % NS) * (L::TILE >> 4);
+                const uint64_t qt = qd + (BK ? 0 : i * (L::TILE >> 4)), kt = kd + (n % NS) * (L::TILE >> 4);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < DB * 4; k++) {
@@ -802,13 +797,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     tc_commit(&sfull[i]);
                 }
             };
-            auto pv = [&](int i, int n, int half) {  // O_i += P_i V_n over 64 keys
+            auto pv = [&](int i, int n, int half, bool add) {  // O_i += P_i V_n over 64 keys
                 const uint64_t vt = vd + (n % NS) * (L::TILE >> 4) + half * (4 * 2048 >> 4);
                 const uint32_t pt = tmem + i * 128 + half * 32;
                 if (elect_one())
 #pragma unroll
                     for (int k = 0; k < 4; k++)
-                        mma_ts(tmem + 256 + i * 128, pt + k * 8, vt + (k * 2048 >> 4), ipv, n + half + k != 0);
+                        mma_ts(tmem + 256 + i * 128, pt + k * 8, vt + (k * 2048 >> 4), ipv, add || half + k != 0);
             };
             auto release = [&](uint64_t *bar) {
                 if (elect_one()) tc_commit(bar);
@@ -818,34 +813,52 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 tc_fence_after();
                 return got;
             };
+            // the query tiles strictly in turn, which keeps one in its softmax while the other multiplies; a
+            // key tile is waited for by its first user and released by its last
             const int nn = j1 - j0;
-            bool ok = wait(&kfull[0], 0);
-            if (ok) {
-                for (int i = 0; i < nq; i++) qk(i, 0);
-                release(&kempty[0]);
-            }
-            // the query tiles strictly in turn, which keeps one in its softmax while the other multiplies
-            for (int n = 0; n < nn && ok; n++) {
-                for (int i = 0; i < nq && ok; i++) {
-                    if (i == 0) ok = wait(&vfull[n % NS], (n / NS) & 1);
+            auto first = [&](int i) { return BK || i == 0; };
+            auto last = [&](int i) { return BK || i == nq - 1; };
+            bool ok = wait(qfull, 0);
+            auto scores = [&](int i, int n) {
+                const int k = key_tile(i, n);
+                if (!ok || k >= nn) return;
+                if (first(i) && !(ok = wait(&kfull[k % NS], (k / NS) & 1))) return;
+                qk(i, k);
+                if (last(i)) release(&kempty[k % NS]);
+            };
+            for (int i = 0; i < nq; i++) scores(i, 0);
+            for (int n = 0; key_tile(0, n) < nn && ok; n++)
+                for (int i = 0; i < nq; i++) {
+                    const int k = key_tile(i, n);
+                    if (k >= nn) break;
+                    if (first(i)) ok = ok && wait(&vfull[k % NS], (k / NS) & 1);
                     for (int h = 0; h < 2 && ok; h++)
-                        if ((ok = wait(&pfull[2 * i + h], n & 1))) pv(i, n, h);
-                    if (ok && n + 1 < nn) {
-                        if (i == 0) ok = wait(&kfull[(n + 1) % NS], ((n + 1) / NS) & 1);
-                        if (!ok) break;
-                        qk(i, n + 1);
-                        if (i == nq - 1) release(&kempty[(n + 1) % NS]);
-                    }
-                    if (i == nq - 1) release(&vempty[n % NS]);
+                        if ((ok = wait(&pfull[2 * i + h], n & 1))) pv(i, k, h, n > 0);
+                    scores(i, n + 1);
+                    if (ok && last(i)) release(&vempty[k % NS]);
                 }
-            }
             release(odone);
             if (!wait(odone, 0) || !ok) s_fail = 1;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        // the query tiles (zero past the rows and D), K-major in the 128B swizzle
+        for (int i = tid - 128; i < (BK ? 1 : nq) * 128 * DB * 8; i += AT_THREADS - 128) {
+            const int r = i / (DB * 8), ch = i % (DB * 8);   // 16-byte chunk of the row
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r0 + r < rows && ch * 8 < c.D) {
+                const int token = (r0 + r) / c.rep, qh = head * c.rep + (r0 + r) - token * c.rep;
+                v = ldg_nc_v4(c.q + token * c.q_stride + (int64_t)qh * c.D + ch * 8);
+            }
+            *reinterpret_cast<uint4 *>(sm + L::Q + (r >> 7) * L::TILE + (ch >> 3) * L::BLOCK + (r & 127) * 128 +
+                                       (((ch & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qfull);
+
         if ((warp - 4) / 4 < nq) {
-        const int wg = (warp - 4) >> 2, row = r0 + wg * 128 + (warp & 3) * 32 + lane;
+        const int wg = (warp - 4) >> 2, trow = (warp & 3) * 32 + lane, row = r0 + (BK ? 0 : wg * 128) + trow;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + wg * 128, to = tmem + lanes + 256 + wg * 128;
         const float s2 = c.scale * LOG2E, slack = 8.0f / s2;
@@ -857,8 +870,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         float m = -INFINITY;
         uint64_t l[2] = {pair2(0.f, 0.f), pair2(0.f, 0.f)};   // the row sum, in four
         bool ok = true;
-        for (int n = 0; n < j1 - j0; n++) {
-            const int s0 = tile_slot(j0 + n);
+        for (int n = 0; key_tile(wg, n) < j1 - j0; n++) {
+            const int k = key_tile(wg, n), s0 = tile_slot(j0 + k);
             uint32_t see[4] = {~0u, ~0u, ~0u, ~0u};
             bool whole = s0 >= sp.b0 && s0 + AT_KT <= sp.b1;
             if (!whole)
@@ -909,19 +922,19 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     }
             }
             // value rows of slots that no row sees: whatever they hold must not meet a zero weight
-            if (wg == 0 && !(s0 >= all.b0 && s0 + AT_KT <= all.b1)) {
-                if (!__all_sync(0xffffffffu, mbar_wait(&vfull[n % NS], (n / NS) & 1))) {
+            if ((BK || wg == 0) && !(s0 >= all.b0 && s0 + AT_KT <= all.b1)) {
+                if (!__all_sync(0xffffffffu, mbar_wait(&vfull[k % NS], (k / NS) & 1))) {
                     s_fail = 1;
                     ok = false;
                     break;
                 }
-                const int x = (warp & 3) * 32 + lane, s = s0 + x;
+                const int s = s0 + trow;
                 if (!(s < all.a1 || (s >= all.c0 && s < all.c1) || (s >= all.b0 && s < all.b1)))
 #pragma unroll
                     for (int b = 0; b < DB; b++)
 #pragma unroll
                         for (int q = 0; q < 8; q++)
-                            *reinterpret_cast<uint4 *>(sm + L::V + (n % NS) * L::TILE + b * L::BLOCK + x * 128 + q * 16) =
+                            *reinterpret_cast<uint4 *>(sm + L::V + (k % NS) * L::TILE + b * L::BLOCK + trow * 128 + q * 16) =
                                 make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
             }
@@ -935,8 +948,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     const int w = 2 * h + x / 16, y = 2 * (x % 16);
                     float e0, e1;
                     unpair2(fma2(pair2(__uint_as_float(v[w][y]), __uint_as_float(v[w][y + 1])), ss, mm), e0, e1);
-                    pk[x] = cvt_bf2(ex2(e0), ex2(e1));
-                    l[x & 1] = add2(l[x & 1], pair2(lo_bf(pk[x]), hi_bf(pk[x])));
+                    e0 = ex2(e0);
+                    e1 = ex2(e1);
+                    pk[x] = cvt_bf2(e0, e1);
+                    l[x & 1] = add2(l[x & 1], pair2(e0, e1));
                 }
                 tmem_st32(ts + 32 * h, pk);
                 tmem_wait_st();
@@ -951,14 +966,47 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             unpair2(add2(l[0], l[1]), lsum, t);
             lsum += t;
         }
-        const bool have = j1 > j0;
+        const bool have = key_tile(wg, 0) < j1 - j0;
         if (ok && have && !__all_sync(0xffffffffu, mbar_wait(odone, 0))) {
             s_fail = 1;
             ok = false;
         }
         tc_fence_after();
+        // by keys: the second half's statistics and O meet the first's through the key and value stages, which
+        // nothing uses any more ([feature][row], then maxima and sums)
+        float *xo = reinterpret_cast<float *>(sm + L::K), *xm = xo + DB * 64 * 128, *xl = xm + 128;
+        float a0 = 1.f, a1 = 0.f;                    // weights of this half's and the other's O
+        const bool two = BK && key_tile(1, 0) < j1 - j0;
+        if (two && wg == 1 && ok) {
+            xm[trow] = m;
+            xl[trow] = lsum;
+#pragma unroll
+            for (int w = 0; w < DB * 2; w++) {
+                uint32_t v[32];
+                tmem_ld32(v, to + 32 * w);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 32; x++) xo[(32 * w + x) * 128 + trow] = __uint_as_float(v[x]);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(xdone);
+        }
+        if (BK && wg == 1) ok = false;        // the first half writes
+        if (two && wg == 0 && ok) {
+            if (!__all_sync(0xffffffffu, mbar_wait(xdone, 0))) {
+                s_fail = 1;
+                ok = false;
+            } else {
+                const float m1 = xm[trow], mm = fmaxf(m, m1);
+                a0 = m == -INFINITY ? 0.f : ex2((m - mm) * s2);
+                a1 = m1 == -INFINITY ? 0.f : ex2((m1 - mm) * s2);
+                lsum = a0 * lsum + a1 * xl[trow];
+                m = mm;
+            }
+        }
         if (ok) {
-            const int64_t prow = (int64_t)token * c.hq + head * c.rep + row % c.rep;
+            const int qh = head * c.rep + row - token * c.rep;
+            const int64_t prow = (int64_t)token * c.hq + qh;
             const bool live = p >= 0;
             const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
             if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? lsum : 0.f);
@@ -970,6 +1018,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     tmem_ld32(v, to + 32 * w);
                     tmem_wait_ld();
                 }
+                if (two)
+#pragma unroll
+                    for (int x = 0; x < 32; x++)
+                        v[x] = __float_as_uint(fmaf(a0, __uint_as_float(v[x]), a1 * xo[(32 * w + x) * 128 + trow]));
                 if (live && have && t.part_o) {
                     float *dst = t.part_o + (blockIdx.z * t.prow + prow) * c.D + 32 * w;
 #pragma unroll
@@ -977,7 +1029,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                         if (32 * w + x < c.D)
                             *reinterpret_cast<uint4 *>(dst + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
                 } else if (live && have) {
-                    uint16_t *dst = c.out + token * c.out_stride + (int64_t)(head * c.rep + row % c.rep) * c.D + 32 * w;
+                    uint16_t *dst = c.out + token * c.out_stride + (int64_t)qh * c.D + 32 * w;
 #pragma unroll
                     for (int x = 0; x < 32; x += 8)
                         if (32 * w + x < c.D) {
@@ -1066,26 +1118,39 @@ static int launch_join(const AttnCall &c, cudaStream_t st) {
     return 0;
 }
 
-template <int DB>
+template <int DB, bool BK>
 static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &mk, const CUtensorMap &mv,
                        cudaStream_t st) {
-    auto kern = attend_tile_kernel<DB>;
+    auto kern = attend_tile_kernel<DB, BK>;
     if (!smem_allowed((const void *)kern, AtLayout<DB>::TOTAL)) return -1;
-    const int64_t pairs = ((int64_t)c.n * c.rep + AT_ROWS - 1) / AT_ROWS;
-    kern<<<dim3((unsigned)pairs, c.hkv, t.splits), AT_THREADS, AtLayout<DB>::TOTAL, st>>>(mk, mv, c, t);
+    const int per = BK ? 128 : AT_ROWS;
+    const int64_t blocks = ((int64_t)c.n * c.rep + per - 1) / per;
+    kern<<<dim3((unsigned)blocks, c.hkv, t.splits), AT_THREADS, AtLayout<DB>::TOTAL, st>>>(mk, mv, c, t);
     MLXD_CHECK(cudaGetLastError());
     return 0;
 }
 
-// key splits of a tile launch: one wave of CTAs when the query tiles alone
-// would leave SMs idle, never more than the key tiles or the workspace's rows
-static int tile_splits(const AttnCall &c, int keys) {
-    const int64_t pairs = ((int64_t)c.n * c.rep + AT_ROWS - 1) / AT_ROWS * c.hkv, rows = (int64_t)c.n * c.hq;
-    int64_t s = num_sms() / pairs;
+// The shape of a tile launch. A CTA of 128 rows whose halves alternate key
+// tiles takes about half the time of one of 256 rows whose halves share every
+// key tile. While the former fit one wave they are taken (a 512-token chunk
+// over a 4096 window 60 us, against 69 in 256 rows and two splits), beyond it
+// the latter, with half the loads per product (a 4096-token chunk 415 us, against
+// 514). Key splits fill the SMs when even those are few, no more than the key
+// tiles or the workspace's rows.
+struct TileShape {
+    int by_keys, splits;
+};
+static TileShape tile_shape(const AttnCall &c, int keys) {
+    const int64_t R = (int64_t)c.n * c.rep, rows = (int64_t)c.n * c.hq, sms = num_sms();
+    const int64_t pairs = (R + AT_ROWS - 1) / AT_ROWS * c.hkv, singles = (R + 127) / 128 * c.hkv;
+    TileShape f;
+    f.by_keys = singles <= sms;
+    int64_t s = sms / (f.by_keys ? singles : pairs);
     if (s > (keys + AT_KT - 1) / AT_KT) s = (keys + AT_KT - 1) / AT_KT;
     if (s > AT_WS_ROWS / rows) s = AT_WS_ROWS / rows;
     if (s > FR_PARTS) s = FR_PARTS;
-    return s < 1 ? 1 : (int)s;
+    f.splits = s < 1 ? 1 : (int)s;
+    return f;
 }
 
 // tail rows of one decode step: sequence blockIdx.x
@@ -1145,21 +1210,26 @@ void kv_attend_prepare(mlxd_kv *kv) {
                row_map(&kv->map_v, kv->v, kv->layers * kv->hkv, kv->cap, kv->d);
 }
 
-static int attend_tiles(AttnCall c, const mlxd_kv *kv, int layer, int splits, bool partial, void *ws, cudaStream_t st) {
+static int attend_tiles(const AttnCall &c, const mlxd_kv *kv, int layer, TileShape shape, bool partial, void *ws,
+                        cudaStream_t st) {
     if (!kv->maps) {
         set_error("attention: the cache has no tensor maps (driver without cuTensorMapEncodeTiled)");
         return -1;
     }
     TileCall t = {};
     t.z0 = layer * kv->hkv;
-    t.splits = splits;
+    t.splits = shape.splits;
     t.prow = (int64_t)c.n * c.hq;
     if (partial) {
         t.part_o = (float *)ws;
         t.part_ml = at_ws_ml(ws, c.D);
     }
     t.fail = fail_word(false);
-    return c.D <= 64 ? launch_tile<1>(c, t, kv->map_k, kv->map_v, st) : launch_tile<2>(c, t, kv->map_k, kv->map_v, st);
+    if (c.D <= 64)
+        return shape.by_keys ? launch_tile<1, true>(c, t, kv->map_k, kv->map_v, st)
+                             : launch_tile<1, false>(c, t, kv->map_k, kv->map_v, st);
+    return shape.by_keys ? launch_tile<2, true>(c, t, kv->map_k, kv->map_v, st)
+                         : launch_tile<2, false>(c, t, kv->map_k, kv->map_v, st);
 }
 
 static int attend_rows(const AttnCall &c, cudaStream_t st) {
@@ -1182,12 +1252,12 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
         set_error("kv_attend: too many query rows");
         return -1;
     }
-    const int splits = tile_splits(c, keys);
-    if (attend_tiles(c, kv, layer, splits, splits > 1, ws, st)) return -1;
-    if (splits == 1) return 0;
+    const TileShape shape = tile_shape(c, keys);
+    if (attend_tiles(c, kv, layer, shape, shape.splits > 1, ws, st)) return -1;
+    if (shape.splits == 1) return 0;
     c.part_o = (const float *)ws;
     c.part_ml = at_ws_ml(ws, c.D);
-    c.parts = splits;
+    c.parts = shape.splits;
     return launch_join(c, st);
 }
 
@@ -1211,11 +1281,11 @@ static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
         b.tk += i * tail;
         b.tv += i * tail;
         if (c.prefix > 0) {
-            const int splits = tile_splits(b, c.prefix);
-            if (attend_tiles(b, kv, layer, splits, true, ws, st)) return -1;
+            const TileShape shape = tile_shape(b, c.prefix);
+            if (attend_tiles(b, kv, layer, shape, true, ws, st)) return -1;
             b.part_o = (const float *)ws;
             b.part_ml = at_ws_ml(ws, c.D);
-            b.parts = splits;
+            b.parts = shape.splits;
         }
         if (attend_few(b, b.rep, c.tcap, c.prefix > 0, nullptr, st)) return -1;
     }
