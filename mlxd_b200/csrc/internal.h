@@ -17,9 +17,9 @@ bool cuda_ok(cudaError_t e, const char *what);
 
 void *dev_alloc(size_t bytes);      // tracked cudaMalloc (nullptr + error on failure)
 void dev_free(void *p);
-// p is memory of the current device (device or managed); false + error naming
-// `what` otherwise (host memory, another device's, null)
-bool on_device(const void *p, const char *what);
+// p is aligned memory of the current device (device or managed); false + error
+// naming `what` otherwise (host memory, another device's, null)
+bool on_device(const void *p, const char *what, int align = 1);
 
 // A projection in device memory. Every quantized matrix keeps its MLX
 // arrays (w u32 [rows][cols/8], scales/biases [rows][cols/group] of sdtype);

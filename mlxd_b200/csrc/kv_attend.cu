@@ -5,6 +5,7 @@
 //
 // over the keys j <= p_i with p_i - j < window or j < sinks, in one pass over
 // the keys with a running maximum m_i.
+#include <limits.h>
 #include <math.h>
 #include <mutex>
 #include <new>
@@ -80,50 +81,6 @@ MLXD_DEV int slot_pos(const AttnCall &c, int s) {
     return last - (d >= 0 ? d : d + ring);
 }
 
-// One warp per (query, head): lane l holds features 8 l .. 8 l + 7; a dot
-// product per key, reduced over the lanes. Serves every head_dim.
-__global__ void __launch_bounds__(128) attend_rows_kernel(AttnCall c) {
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= (int64_t)c.n * c.hq) return;
-    const int i = (int)(row / c.hq), h = (int)(row % c.hq), g = h / c.rep;
-    if (c.lens && c.lens[i] < 0) return;
-    const int p = query_pos(c, i);
-    const bool mine = lane * 8 < c.D;
-    float q[8], acc[8], m = -INFINITY, l = 0.f;
-    for (int d = 0; d < 8; d++) {
-        q[d] = mine ? bf2f(c.q[i * c.q_stride + (int64_t)h * c.D + lane * 8 + d]) * c.scale : 0.f;
-        acc[d] = 0.f;
-    }
-    const int lo = window_lo(c, p), head = min(c.sinks, lo);   // sinks before the window
-    for (int t = 0; t < head + p + 1 - lo; t++) {
-        const int j = t < head ? t : lo + t - head;
-        const uint16_t *kr, *vr;
-        if (c.lens && j >= c.prefix) {
-            const int64_t o = (((int64_t)i * c.hkv + g) * c.tcap + (j - c.prefix)) * c.D;
-            kr = c.tk + o;
-            vr = c.tv + o;
-        } else {
-            const int s = j < c.cap ? j : c.ring_sinks + (j - c.ring_sinks) % (c.cap - c.ring_sinks);
-            const int64_t o = ((int64_t)g * c.cap + s) * c.D;
-            kr = c.k + o;
-            vr = c.v + o;
-        }
-        float z = 0.f;
-        if (mine)
-            for (int d = 0; d < 8; d++) z = fmaf(q[d], bf2f(kr[lane * 8 + d]), z);
-        z = warp_sum(z);
-        const float mn = fmaxf(m, z), a = mn == -INFINITY ? 1.f : expf(m - mn), e = mn == -INFINITY ? 0.f : expf(z - mn);
-        m = mn;
-        l = fmaf(l, a, e);
-        if (mine)
-            for (int d = 0; d < 8; d++) acc[d] = fmaf(acc[d], a, e * bf2f(vr[lane * 8 + d]));
-    }
-    if (mine)
-        for (int d = 0; d < 8; d++)
-            c.out[i * c.out_stride + (int64_t)h * c.D + lane * 8 + d] = f2bf(l > 0.f ? acc[d] / l : l);
-}
-
 // the partial results' room in a workspace: 148 CTAs of 256 rows, whatever
 // the call (more rows than that go unsplit, or in batches)
 constexpr int64_t AT_WS_ROWS = 148 * 256;
@@ -157,6 +114,7 @@ constexpr int FR_MAXCL = 8;                        // CTAs of a cluster (the por
 constexpr int FR_PARTS = 56, FR_SRC = 64;          // splits of a prefix, and those with a cluster's CTAs
 
 struct FewCall {
+    int tails;                 // an item is one sequence's tail, else up to ROWS query rows over the cache
     int cluster;               // grid x is a cluster whose results meet, else each CTA's is partial
     float *part_o;             // partial results [grid x][prow], or null: the whole result to out
     float2 *part_ml;
@@ -189,61 +147,36 @@ __global__ void __launch_bounds__(W * 32)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, cc = lane & 3;
     const int rank = blockIdx.x, ncta = gridDim.x;   // the item's CTAs
     const int head = blockIdx.y % c.hkv, tile = blockIdx.y / c.hkv, seq = blockIdx.z;
-    const int rows_total = c.lens ? c.rep : c.n * c.rep, r0 = tile * ROWS, nrows = min(ROWS, rows_total - r0);
-    auto token_of = [&](int r) { return c.lens ? seq : (r0 + r) / c.rep; };
-    auto qhead_of = [&](int r) { return head * c.rep + (c.lens || c.n == 1 ? r0 + r : (r0 + r) % c.rep); };
-    pdl_trigger();                                 // the join kernel may be put in place
-    if (c.lens && c.lens[seq] < 0) return;         // a finished sequence: the whole cluster
+    const int rows_total = t.tails ? c.rep : c.n * c.rep, r0 = tile * ROWS, nrows = min(ROWS, rows_total - r0);
+    const bool one = t.tails || c.n == 1;            // the rows are heads of one token
+    auto token_of = [&](int r) { return t.tails ? seq : one ? 0 : (r0 + r) / c.rep; };
+    auto qhead_of = [&](int r) { return head * c.rep + (one ? r0 + r : (r0 + r) % c.rep); };
+    pdl_trigger();                                 // the kernel that joins may be put in place
+    if (t.tails && c.lens[seq] < 0) return;        // a finished sequence: the whole cluster
 
-    // the item's keys
-    const int pmin = query_pos(c, token_of(0)), pmax = query_pos(c, token_of(nrows - 1));
-    Span sp;
+    // positions of the rows (lane r: row r; -1: not asked) and the item's keys
+    const int rp = lane < nrows ? query_pos(c, token_of(lane)) : -1;
+    const int pmax = __reduce_max_sync(0xffffffffu, rp);
+    const int pmin = __reduce_min_sync(0xffffffffu, rp < 0 ? INT32_MAX : rp);
+    const bool multi = __any_sync(0xffffffffu, lane < nrows && rp != pmax);   // masks per row
+    Span sp = {0, 0, 0, 0, 0};
     const uint16_t *kb, *vb;
-    if (c.lens) {
+    if (t.tails) {
         const int lo = window_lo(c, pmax);
         sp.a1 = max(0, min(c.sinks, lo) - c.prefix);
-        sp.c0 = sp.c1 = 0;
         sp.b0 = max(0, lo - c.prefix);
         sp.b1 = pmax + 1 - c.prefix;
         const size_t o = ((size_t)seq * c.hkv + head) * c.tcap * c.D;
         kb = c.tk + o;
         vb = c.tv + o;
     } else {
-        sp = span_of(c, window_lo(c, pmin), pmax + 1);
+        if (pmax >= 0) sp = span_of(c, window_lo(c, pmin), pmax + 1);
         kb = c.k + (size_t)head * c.cap * c.D;
         vb = c.v + (size_t)head * c.cap * c.D;
     }
     const int na = (sp.a1 + 15) / 16, nc = (max(0, sp.c1 - sp.c0) + 15) / 16, nb = (max(0, sp.b1 - sp.b0) + 15) / 16;
     const int ns = na + nc + nb, wg = rank * W + warp, nwg = ncta * W;
     const int st0 = (int)((int64_t)ns * wg / nwg), st1 = (int)((int64_t)ns * (wg + 1) / nwg);
-
-    // query fragments: column g (of each column tile), features in the keys' order
-    uint4 qb[NT][NU];
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-        const int r = ROWS == 4 ? g & 3 : g + 8 * i;
-        const uint16_t *q = c.q + token_of(r) * c.q_stride + (int64_t)qhead_of(r) * c.D + 8 * cc;
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-            qb[i][u] = r < nrows && 32 * u + 8 * cc < c.D ? ldg_nc_v4(q + 32 * u) : make_uint4(0, 0, 0, 0);
-    }
-    // this lane's columns 2 cc and 2 cc + 1 of a column tile: rows, positions, statistics
-    auto row_of = [&](int i, int x) { return ROWS == 4 ? (2 * cc + x) & 3 : 8 * i + 2 * cc + x; };
-    const bool multi = pmin != pmax;               // rows at several positions: masks per row
-    int p[NT][2];
-    float m[NT][2], l[NT][2], o[NT][NW * 4][4];
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            p[i][x] = multi && row_of(i, x) < nrows ? query_pos(c, token_of(row_of(i, x))) : pmax;
-            m[i][x] = -INFINITY;
-            l[i][x] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < NW * 4; j++) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
-    }
-    const float s2 = c.scale * LOG2E;
 
     auto step_slots = [&](int st, int &s, int &e) {
         const bool a = st < na, b = st >= na + nc;
@@ -255,9 +188,7 @@ __global__ void __launch_bounds__(W * 32)
     constexpr int KV = 2 * NU + 4 * NW;              // 16-byte pieces of a lane per step
     uint4 *ring = reinterpret_cast<uint4 *>(fsm) + (size_t)warp * FR_DEPTH * KV * 32 + lane;
     int put = 0, get = 0;                            // ring stages
-#pragma unroll 1
-    for (int st = st0 - (FR_DEPTH - 1); st < st1; st++) {
-        const int ahead = st + FR_DEPTH - 1;
+    auto fetch = [&](int ahead) {
         if (ahead < st1) {
             int s, e;
             step_slots(ahead, s, e);
@@ -284,7 +215,41 @@ __global__ void __launch_bounds__(W * 32)
             }
         }
         cp_async_commit();
-        if (st < st0) continue;                      // the ring's first stages
+    };
+#pragma unroll 1
+    for (int i = 0; i < FR_DEPTH - 1; i++) fetch(st0 + i);
+
+    // query fragments: column g (of each column tile), features in the keys' order
+    uint4 qb[NT][NU];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+        const int r = ROWS == 4 ? g & 3 : g + 8 * i;
+        const uint16_t *q = c.q + token_of(r) * c.q_stride + (int64_t)qhead_of(r) * c.D + 8 * cc;
+#pragma unroll
+        for (int u = 0; u < NU; u++)
+            qb[i][u] = r < nrows && 32 * u + 8 * cc < c.D ? ldg_nc_v4(q + 32 * u) : make_uint4(0, 0, 0, 0);
+    }
+    // this lane's columns 2 cc and 2 cc + 1 of a column tile: rows, positions, statistics
+    auto row_of = [&](int i, int x) { return ROWS == 4 ? (2 * cc + x) & 3 : 8 * i + 2 * cc + x; };
+    int p[NT][2];
+    float m[NT][2], l[NT][2], o[NT][NW * 4][4];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            const int r = row_of(i, x), at = __shfl_sync(0xffffffffu, rp, r);
+            p[i][x] = r < nrows ? at : pmax;
+            m[i][x] = -INFINITY;
+            l[i][x] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NW * 4; j++) o[i][j][0] = o[i][j][1] = o[i][j][2] = o[i][j][3] = 0.f;
+    }
+    const float s2 = c.scale * LOG2E;
+
+#pragma unroll 1
+    for (int st = st0; st < st1; st++) {
+        fetch(st + FR_DEPTH - 1);
         cp_async_wait<FR_DEPTH - 1>();
         const uint4 *src = ring + get * KV * 32;
         get = get + 1 == FR_DEPTH ? 0 : get + 1;
@@ -540,7 +505,7 @@ static int launch_few(const AttnCall &c, const FewCall &t, int splits, int tiles
     const size_t smem = ((size_t)W * (fr_warp_floats(NU, ROWS) + 2 * ROWS) + (FR_SRC + 1) * ROWS) * 4;
     if (!smem_allowed((const void *)kern, smem)) return -1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(splits, c.hkv * tiles, c.lens ? c.n : 1);
+    cfg.gridDim = dim3(splits, c.hkv * tiles, t.tails ? c.n : 1);
     cfg.blockDim = dim3(W * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -571,6 +536,10 @@ static int launch_few_rows(const AttnCall &c, const FewCall &t, int R, int split
 }
 template <int W>
 static int launch_few_w(const AttnCall &c, const FewCall &t, int R, int splits, int tiles, bool pdl, cudaStream_t st) {
+    if constexpr (W == 4) {                          // (8 such rings exceed an SM's shared memory)
+        if (c.D > 192) return launch_few_rows<8, 4>(c, t, R, splits, tiles, pdl, st);
+        if (c.D > 128) return launch_few_rows<6, 4>(c, t, R, splits, tiles, pdl, st);
+    }
     switch ((c.D + 31) / 32) {
     case 1: return launch_few_rows<1, W>(c, t, R, splits, tiles, pdl, st);
     case 2: return launch_few_rows<2, W>(c, t, R, splits, tiles, pdl, st);
@@ -583,37 +552,48 @@ static int launch_few_w(const AttnCall &c, const FewCall &t, int R, int splits, 
 
 static int launch_join(const AttnCall &c, cudaStream_t st);
 
-// rows: query rows of an item that share a kv head; keys: the most that an
-// item reads; ws: room for partial results (null: none are made)
-static int attend_few(AttnCall c, int rows, int keys, bool pdl, void *ws, cudaStream_t st) {
-    const int R = rows > 8 ? 16 : rows > 4 ? 8 : 4, tiles = (rows + R - 1) / R;
-    if ((int64_t)c.hkv * tiles > 65535 || (c.lens && c.n > 65535)) {
+// What a few-rows launch is for: the whole result of a cache call; a prefix's
+// partial results for a group (into c.part_*); tails, which join them.
+enum FewKind { FEW_CACHE, FEW_PREFIX, FEW_TAILS };
+
+// keys: the most that an item reads
+static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_t st) {
+    const int64_t rows = kind == FEW_TAILS ? c.rep : (int64_t)c.n * c.rep, qrows = (int64_t)c.n * c.hq;
+    const int R = rows > 8 ? 16 : rows > 4 ? 8 : 4;
+    const int64_t tiles = (rows + R - 1) / R, items = c.hkv * tiles * (kind == FEW_TAILS ? c.n : 1);
+    if (c.hkv * tiles > 65535 || c.n > 65535) {
         set_error("attention: too many rows for one launch");
         return -1;
     }
-    const int64_t items = (int64_t)c.hkv * tiles * (c.lens ? c.n : 1);
     FewCall t = {};
-    // CTAs per item: as many as fill the SMs while each of their 8 warps has two steps of 16 keys
-    int64_t s = num_sms() / items, most = (keys + 8 * 32 - 1) / (8 * 32);
-    if (s > most) s = most;
+    t.tails = kind == FEW_TAILS;
+    // CTAs per item: as many as fill the SMs while each of their warps has two steps of 16 keys
+    const int W = c.D > 128 || items >= num_sms() ? 4 : 8;   // items enough: two CTAs to an SM
+    int64_t s = num_sms() / items;
+    if (s > (keys + W * 32 - 1) / (W * 32)) s = (keys + W * 32 - 1) / (W * 32);
     if (s > FR_PARTS) s = FR_PARTS;
-    if (s > AT_WS_ROWS / ((int64_t)c.n * c.hq)) s = AT_WS_ROWS / ((int64_t)c.n * c.hq);
-    if (s > 2 * FR_MAXCL && ws) {
-        // more than two clusters' worth: partial results and a second kernel
-        t.prow = (int64_t)c.n * c.hq;
+    if (s > AT_WS_ROWS / qrows) s = AT_WS_ROWS / qrows;
+    if (s < 1) s = 1;
+    // more than two clusters' worth: partial results and a second kernel
+    const bool partial = kind == FEW_PREFIX || (kind == FEW_CACHE && s > 2 * FR_MAXCL);
+    if (partial) {
+        t.prow = qrows;
         t.part_o = (float *)ws;
         t.part_ml = at_ws_ml(ws, c.D);
-        if (launch_few_w<8>(c, t, R, (int)s, tiles, pdl, st)) return -1;
-        c.part_o = t.part_o;
-        c.part_ml = t.part_ml;
-        c.parts = (int)s;
-        return launch_join(c, st);
+    } else {
+        int cl = 1;
+        while (cl < FR_MAXCL && cl * 2 <= s) cl *= 2;
+        s = cl;
+        t.cluster = cl > 1;
     }
-    int cl = 1;
-    while (cl < FR_MAXCL && cl * 2 <= s) cl *= 2;
-    t.cluster = cl > 1;
-    // items enough for every SM: CTAs of 4 warps, two to an SM
-    return items >= num_sms() ? launch_few_w<4>(c, t, R, cl, tiles, pdl, st) : launch_few_w<8>(c, t, R, cl, tiles, pdl, st);
+    const bool pdl = kind == FEW_TAILS && c.parts > 0;
+    if (W == 4 ? launch_few_w<4>(c, t, R, (int)s, (int)tiles, pdl, st) : launch_few_w<8>(c, t, R, (int)s, (int)tiles, pdl, st))
+        return -1;
+    if (!partial) return 0;
+    c.part_o = t.part_o;
+    c.part_ml = t.part_ml;
+    c.parts = (int)s;
+    return kind == FEW_CACHE ? launch_join(c, st) : 0;
 }
 
 // ---- many query rows per kv head: tensor-core tiles
@@ -1076,32 +1056,33 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
         L = fmaf(w[u], ml[u].y, L);
     }
     L = warp_sum(L);
-    const int d = lane * 4;
-    const float *po = c.part_o + row * c.D + d;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < c.parts; k += 4) {
-        float4 v[4];
-        float a[4];
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const float lo = __shfl_sync(0xffffffffu, w[0], (k + u) & 31), hi = __shfl_sync(0xffffffffu, w[1], (k + u) & 31);
-            a[u] = k + u >= c.parts ? 0.f : k + u < 32 ? lo : hi;
-            // a split that saw nothing wrote no row
-            v[u] = d < c.D && a[u] != 0.f ? *reinterpret_cast<const float4 *>(po + (k + u) * prow * c.D)
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-            acc.x = fmaf(a[u], v[u].x, acc.x);
-            acc.y = fmaf(a[u], v[u].y, acc.y);
-            acc.z = fmaf(a[u], v[u].z, acc.z);
-            acc.w = fmaf(a[u], v[u].w, acc.w);
-        }
-    }
     const float inv = L > 0.f ? 1.0f / L : 0.f;
-    if (d < c.D)
-        *reinterpret_cast<uint2 *>(c.out + row / c.hq * c.out_stride + row % c.hq * c.D + d) =
-            make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
+    for (int d = lane * 4; d - lane * 4 < c.D; d += 128) {
+        const float *po = c.part_o + row * c.D + d;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < c.parts; k += 4) {       // four loads in flight
+            float4 v[4];
+            float a[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float lo = __shfl_sync(0xffffffffu, w[0], (k + u) & 31), hi = __shfl_sync(0xffffffffu, w[1], (k + u) & 31);
+                a[u] = k + u >= c.parts ? 0.f : k + u < 32 ? lo : hi;
+                // a split that saw nothing wrote no row
+                v[u] = d < c.D && a[u] != 0.f ? *reinterpret_cast<const float4 *>(po + (k + u) * prow * c.D)
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                acc.x = fmaf(a[u], v[u].x, acc.x);
+                acc.y = fmaf(a[u], v[u].y, acc.y);
+                acc.z = fmaf(a[u], v[u].z, acc.z);
+                acc.w = fmaf(a[u], v[u].w, acc.w);
+            }
+        }
+        if (d < c.D)
+            *reinterpret_cast<uint2 *>(c.out + row / c.hq * c.out_stride + row % c.hq * c.D + d) =
+                make_uint2(cvt_bf2(acc.x * inv, acc.y * inv), cvt_bf2(acc.z * inv, acc.w * inv));
+    }
 }
 
 static int launch_join(const AttnCall &c, cudaStream_t st) {
@@ -1232,39 +1213,40 @@ static int attend_tiles(const AttnCall &c, const mlxd_kv *kv, int layer, TileSha
                          : launch_tile<2, false>(c, t, kv->map_k, kv->map_v, st);
 }
 
-static int attend_rows(const AttnCall &c, cudaStream_t st) {
-    const int64_t rows = (int64_t)c.n * c.hq;
-    if ((rows + 3) / 4 > INT32_MAX) {
-        set_error("attention: too many query rows");
-        return -1;
+static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
+    const int64_t span = (int64_t)c.window + c.n - 1 + c.sinks, rows = (int64_t)c.n * c.rep;
+    const int keys = c.window && span < c.total ? (int)span : c.total;   // the most that one row group sees
+    if (c.D <= 128 && rows > 16 && c.n > 1) {
+        if (rows > INT_MAX - AT_ROWS || c.hkv > 65535) {
+            set_error("kv_attend: too many query rows");
+            return -1;
+        }
+        const TileShape shape = tile_shape(c, keys);
+        if (attend_tiles(c, kv, layer, shape, shape.splits > 1, ws, st)) return -1;
+        if (shape.splits == 1) return 0;
+        c.part_o = (const float *)ws;
+        c.part_ml = at_ws_ml(ws, c.D);
+        c.parts = shape.splits;
+        return launch_join(c, st);
     }
-    attend_rows_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, st>>>(c);
-    MLXD_CHECK(cudaGetLastError());
+    // few rows, or heads too wide for the tiles' accumulators: tokens in launches of at most 65535 items
+    int64_t most = (int64_t)(65535 / c.hkv) * 16 / c.rep;
+    most = most < 1 ? 1 : most > 65535 ? 65535 : most;
+    const int n = c.n;
+    for (int i = 0; i < n; i += (int)most) {
+        AttnCall b = c;
+        b.n = n - i < most ? n - i : (int)most;
+        b.q += i * c.q_stride;
+        b.out += i * c.out_stride;
+        b.pos0 += i;
+        if (attend_few(b, FEW_CACHE, keys, ws, st)) return -1;
+    }
     return 0;
 }
 
-static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
-    if (c.D > 128) return attend_rows(c, st);
-    const int64_t span = (int64_t)c.window + c.n - 1 + c.sinks;
-    const int keys = c.window && span < c.total ? (int)span : c.total;   // the most that one row group sees
-    if ((int64_t)c.n * c.rep <= 16 || c.n == 1) return attend_few(c, c.n * c.rep, keys, false, ws, st);
-    if ((int64_t)c.n * c.rep > INT32_MAX - AT_ROWS || c.hkv > 65535) {
-        set_error("kv_attend: too many query rows");
-        return -1;
-    }
-    const TileShape shape = tile_shape(c, keys);
-    if (attend_tiles(c, kv, layer, shape, shape.splits > 1, ws, st)) return -1;
-    if (shape.splits == 1) return 0;
-    c.part_o = (const float *)ws;
-    c.part_ml = at_ws_ml(ws, c.D);
-    c.parts = shape.splits;
-    return launch_join(c, st);
-}
-
-// sequences in batches whose partial rows fit the workspace: the prefix on
-// tiles, then every sequence's tail, which joins the prefix's results
+// sequences in batches whose partial rows fit the workspace: the prefix (on
+// tiles unless the heads are too wide), then every sequence's tail, which joins the prefix's results
 static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
-    if (c.D > 128) return attend_rows(c, st);
     const int64_t tail = (int64_t)c.hkv * c.tcap * c.D;
     int64_t most = AT_WS_ROWS / c.hq < 65535 ? AT_WS_ROWS / c.hq : 65535;
     if (most < 1) {
@@ -1280,14 +1262,16 @@ static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
         b.lens += i;
         b.tk += i * tail;
         b.tv += i * tail;
-        if (c.prefix > 0) {
+        if (c.prefix > 0 && c.D > 128) {
+            if (attend_few(b, FEW_PREFIX, c.prefix, ws, st)) return -1;
+        } else if (c.prefix > 0) {
             const TileShape shape = tile_shape(b, c.prefix);
             if (attend_tiles(b, kv, layer, shape, true, ws, st)) return -1;
             b.part_o = (const float *)ws;
             b.part_ml = at_ws_ml(ws, c.D);
             b.parts = shape.splits;
         }
-        if (attend_few(b, b.rep, c.tcap, c.prefix > 0, nullptr, st)) return -1;
+        if (attend_few(b, FEW_TAILS, c.tcap, nullptr, st)) return -1;
     }
     return 0;
 }
@@ -1312,7 +1296,8 @@ static int attn_call(AttnCall &c, const char *what, int hkv, int D, const void *
         set_error("%s: workspace too small or misaligned", what);
         return -1;
     }
-    if (!on_device(q, "attention: q") || !on_device(out, "attention: out") || !on_device(ws, "attention: workspace"))
+    if (!on_device(q, "attention: q", 16) || !on_device(out, "attention: out", 16) ||
+        !on_device(ws, "attention: workspace", 256))
         return -1;
     c.q = (const uint16_t *)q;
     c.out = (uint16_t *)out;
@@ -1455,7 +1440,7 @@ int mlxd_cuda_kv_group_append(mlxd_kv_group *g, int layer, const void *k, int64_
         return -1;
     }
     if (!on_device(k, "kv_group_append: k") || !on_device(v, "kv_group_append: v") ||
-        !on_device(lens_dev, "kv_group_append: lengths") || !same_device(g->device, "kv_group_append"))
+        !on_device(lens_dev, "kv_group_append: lengths", 4) || !same_device(g->device, "kv_group_append"))
         return -1;
     const size_t o = (size_t)layer * g->n * g->hkv * g->cap * g->d;
     group_append_kernel<<<g->n, 128, 0, (cudaStream_t)stream>>>((const uint16_t *)k, k_stride, (const uint16_t *)v,
@@ -1474,7 +1459,7 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     }
     AttnCall c = {};
     if (attn_call(c, "kv_group_attend", g->hkv, g->d, q, q_stride, g->n, a, out, out_stride, ws, ws_bytes) ||
-        !on_device(lens_dev, "kv_group_attend: lengths") || !same_device(g->device, "kv_group_attend") ||
+        !on_device(lens_dev, "kv_group_attend: lengths", 4) || !same_device(g->device, "kv_group_attend") ||
         gave_up("kv_group_attend"))
         return -1;
     const size_t layer_elems = (size_t)g->hkv * g->prefix->cap * g->d;

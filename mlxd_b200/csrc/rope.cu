@@ -202,9 +202,15 @@ extern "C" int mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int he
         set_error("rope: bad arguments (dims: even, at most head_dim <= 256)");
         return -1;
     }
-    if (x_token_stride < 0 || x_head_stride < 0 || y_token_stride < 0 || y_head_stride < head_dim ||
-        (n > 1 && y_token_stride < head_dim)) {
-        set_error("rope: rows of y overlap");
+    // y's rows do not overlap: heads within a token's span, or tokens within a head's
+    const int64_t D = head_dim, most = INT64_MAX / 4 / ((int64_t)n + heads);
+    const bool in_range = x_token_stride >= 0 && x_head_stride >= 0 && y_token_stride >= 0 && y_head_stride >= 0 &&
+                          x_token_stride <= most && x_head_stride <= most && y_token_stride <= most && y_head_stride <= most;
+    if (!in_range || !(((heads == 1 || y_head_stride >= D) &&
+                        (n <= 1 || y_token_stride - D >= (heads - 1) * y_head_stride)) ||
+                       ((n <= 1 || y_token_stride >= D) &&
+                        (heads == 1 || y_head_stride - D >= (n - 1) * y_token_stride)))) {
+        set_error("rope: rows of y overlap, or a stride out of range");
         return -1;
     }
     if (!pos_dev && (int64_t)pos + n > INT32_MAX) {
@@ -212,10 +218,11 @@ extern "C" int mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int he
         return -1;
     }
     if (n == 0) return 0;
+    const int elem = dtype == MLXD_BF16 ? 2 : 4;
     RopeCall c;
     c.dims = r->dims;
-    if (rope_turns(*r, c) || !on_device(x, "rope: x") || !on_device(y, "rope: y") ||
-        (pos_dev && !on_device(pos_dev, "rope: positions")))
+    if (rope_turns(*r, c) || !on_device(x, "rope: x", elem) || !on_device(y, "rope: y", elem) ||
+        (pos_dev && !on_device(pos_dev, "rope: positions", 4)))
         return -1;
     c.x = x;
     c.y = y;

@@ -58,11 +58,15 @@ void dev_free(void *p) {
     cudaFree(p);
 }
 
-bool on_device(const void *p, const char *what) {
+bool on_device(const void *p, const char *what, int align) {
     int dev = 0;
     cudaPointerAttributes a;
     if (!p) {
         set_error("%s: null pointer", what);
+        return false;
+    }
+    if ((uintptr_t)p % align) {
+        set_error("%s: not aligned to %d bytes", what, align);
         return false;
     }
     if (!cuda_ok(cudaGetDevice(&dev), what) || !cuda_ok(cudaPointerGetAttributes(&a, p), what)) return false;

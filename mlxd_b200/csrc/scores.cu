@@ -564,16 +564,13 @@ extern "C" int mlxd_cuda_token_scores(const void *logits, int dtype, int rows, i
         set_error("token_scores: logprobs without targets");
         return -1;
     }
-    if ((uintptr_t)logits % (dtype == MLXD_BF16 ? 2 : 4)) {
-        set_error("token_scores: misaligned logits");
-        return -1;
-    }
     if (rows == 0) return 0;
-    if (!on_device(logits, "token_scores: logits") || (targets && !on_device(targets, "token_scores: targets")) ||
-        (logprobs && !on_device(logprobs, "token_scores: logprobs")) ||
-        (entropy && !on_device(entropy, "token_scores: entropy")) ||
-        (n_top && top_ids && !on_device(top_ids, "token_scores: top ids")) ||
-        (n_top && top_logprobs && !on_device(top_logprobs, "token_scores: top logprobs")))
+    if (!on_device(logits, "token_scores: logits", dtype == MLXD_BF16 ? 2 : 4) ||
+        (logprobs && !on_device(targets, "token_scores: targets", 4)) ||
+        (logprobs && !on_device(logprobs, "token_scores: logprobs", 4)) ||
+        (entropy && !on_device(entropy, "token_scores: entropy", 4)) ||
+        (n_top && top_ids && !on_device(top_ids, "token_scores: top ids", 4)) ||
+        (n_top && top_logprobs && !on_device(top_logprobs, "token_scores: top logprobs", 4)))
         return -1;
     const ScoreCall c = {logits, row_stride, rows, V, n_top, targets, logprobs, entropy, top_logprobs, top_ids};
     return dtype == MLXD_BF16 ? launch_scores<uint16_t>(c, (cudaStream_t)stream)

@@ -30,7 +30,9 @@ def test_rope_refuses_bad_shapes(kw):
     refused(rope(**kw), "rope: bad arguments")
 
 
-@pytest.mark.parametrize("kw", [dict(ys=(8, 4), heads=2), dict(ys=(4, 8), n=2), dict(xs=(-8, 8)), dict(ys=(-8, 8))])
+@pytest.mark.parametrize("kw", [dict(ys=(8, 4), heads=2), dict(ys=(4, 8), n=2), dict(xs=(-8, 8)), dict(ys=(-8, 8)),
+                                dict(ys=(8, 8), n=2, heads=2), dict(ys=(20, 12), n=2, heads=3),
+                                dict(ys=(8, 2 ** 62), heads=3)])
 def test_rope_refuses_strides(kw):
     refused(rope(**kw), "rows of y overlap")
 

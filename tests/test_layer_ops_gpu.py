@@ -407,7 +407,7 @@ class Cache:
 
 
 @pytest.mark.parametrize("hkv,rep,D", [(2, 4, 128), (1, 8, 64), (3, 1, 80), (2, 7, 96), (1, 32, 128), (2, 2, 16),
-                                       (1, 3, 8), (2, 5, 256), (2, 16, 64), (1, 2, 136)])
+                                       (1, 3, 8), (2, 5, 256), (2, 16, 64), (1, 2, 136), (1, 4, 192)])
 @pytest.mark.parametrize("n,pos", [(1, 0), (1, 63), (1, 300), (1, 2191), (2, 0), (5, 127), (33, 96), (130, 0),
                                    (300, 517)])
 def test_attend(gen, n, pos, hkv, rep, D):
@@ -445,6 +445,15 @@ def test_attend_large_chunk(gen):
     c = Cache(gen, 2, 128, 3000, 3000, layers=1, layer=0)
     q = rand(gen, 1777, 16, 128, scale=1.5)
     c.check(c.attend(q, 1223, cuda.attn_config(16)), q, 1223, heads=[0, 9, 15])
+
+
+def test_attend_wide_heads_long(gen):
+    """Head dim 256: a single token over a long cache (split and joined), a chunk in several launches' worth of rows."""
+    c = Cache(gen, 2, 256, 9000, 9000, layers=1, layer=0)
+    q = rand(gen, 1, 16, 256, scale=1.5)
+    c.check(c.attend(q, 8999, cuda.attn_config(16)), q, 8999, heads=[0, 9])
+    q = rand(gen, 700, 16, 256, scale=1.5)
+    c.check(c.attend(q, 5000, cuda.attn_config(16)), q, 5000, heads=[3, 15])
 
 
 @pytest.mark.parametrize("n", [1, 40, 200])
@@ -557,6 +566,14 @@ def test_attend_refusals(gen):
     assert rc == -1 and b"not held" in L.mlxd_cuda_last_error()     # past the end of a cache that is no ring
     assert L.mlxd_cuda_kv_attend(flat.kv, 0, q.data_ptr(), 256, 0, 0, C.byref(cuda.attn_config(4)), out.data_ptr(),
                                  256, ws.data_ptr(), ws.numel(), None) == 0
+    odd = lambda x=0, y=0, p=0: L.mlxd_cuda_rope(q.data_ptr() + x, cuda.BF16, 1, 4, 64, 256, 64, C.byref(  # noqa: E731
+        cuda.rope_config(1e4, 64)), ws.data_ptr() + 256 + p, 0, out.data_ptr() + y, 256, 64, None)
+    for kw in (dict(x=1), dict(y=1), dict(p=2)):
+        assert odd(**kw) == -1 and b"not aligned" in L.mlxd_cuda_last_error()
+    lg = lambda x=0, t=0, o=0: L.mlxd_cuda_token_scores(q.data_ptr() + x, cuda.F32, 1, 64, 64, ws.data_ptr() + t, 0,  # noqa: E731
+                                                        out.data_ptr() + o, None, None, None, None)
+    for kw in (dict(x=2), dict(t=1), dict(o=2)):
+        assert lg(**kw) == -1 and b"not aligned" in L.mlxd_cuda_last_error()
     assert L.mlxd_cuda_rope(q.data_ptr(), cuda.BF16, 1, 4, 64, 256, 64, C.byref(cuda.rope_config(1e4, 64)), None, 0,
                             aligned, 256, 64, None) == -1
     assert b"not device memory" in L.mlxd_cuda_last_error()
