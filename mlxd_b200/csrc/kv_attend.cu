@@ -822,16 +822,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        // the query tiles (zero past the rows and D), K-major in the 128B swizzle
-        for (int i = tid - 128; i < (BK ? 1 : nq) * 128 * DB * 8; i += AT_THREADS - 128) {
-            const int r = i / (DB * 8), ch = i % (DB * 8);   // 16-byte chunk of the row
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r0 + r < rows && ch * 8 < c.D) {
-                const int token = (r0 + r) / c.rep, qh = head * c.rep + (r0 + r) - token * c.rep;
-                v = ldg_nc_v4(c.q + token * c.q_stride + (int64_t)qh * c.D + ch * 8);
+        // the query tiles (zero past the rows and D), K-major in the 128B swizzle: a warp's rows, whose addresses
+        // its lanes hold, in 16-byte chunks with all loads in flight
+        {
+            constexpr int RW = (BK ? 128 : AT_ROWS) / 8, PER = RW * DB / 4;
+            const int w0 = (warp - 4) * RW, mine = r0 + w0 + lane, tok = mine / c.rep;
+            const uint16_t *src = c.q + tok * c.q_stride + (int64_t)(head * c.rep + mine - tok * c.rep) * c.D;
+            uint4 v[PER];
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int r = i * (4 / DB) + lane / (DB * 8), ch = lane % (DB * 8);
+                const uint16_t *at = reinterpret_cast<const uint16_t *>(__shfl_sync(0xffffffffu, (unsigned long long)src, r));
+                v[i] = r0 + w0 + r < rows && ch * 8 < c.D ? ldg_nc_v4(at + ch * 8) : make_uint4(0, 0, 0, 0);
             }
-            *reinterpret_cast<uint4 *>(sm + L::Q + (r >> 7) * L::TILE + (ch >> 3) * L::BLOCK + (r & 127) * 128 +
-                                       (((ch & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int r = w0 + i * (4 / DB) + lane / (DB * 8), ch = lane % (DB * 8);
+                *reinterpret_cast<uint4 *>(sm + L::Q + (r >> 7) * L::TILE + (ch >> 3) * L::BLOCK + (r & 127) * 128 +
+                                           (((ch & 7) ^ (r & 7)) << 4)) = v[i];
+            }
         }
         fence_proxy_async();
         __syncwarp();
@@ -988,37 +997,40 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             const int qh = head * c.rep + row - token * c.rep;
             const int64_t prow = (int64_t)token * c.hq + qh;
             const bool live = p >= 0;
-            const float inv = lsum > 0.f ? 1.0f / lsum : 0.f;
+            const float inv = t.part_o ? 1.f : lsum > 0.f ? 1.0f / lsum : 0.f;
             if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? lsum : 0.f);
-#pragma unroll
-            for (int w = 0; w < DB * 2; w++) {
+            // 32 columns at a time through shared memory (rows of 36 floats, in the value stages), so that 8
+            // lanes write one row's
+            float *stage = reinterpret_cast<float *>(sm + L::V + 4096) + (warp - 4) * 32 * 36;
+            char *dst = t.part_o ? reinterpret_cast<char *>(t.part_o + (blockIdx.z * t.prow + prow) * c.D)
+                                 : reinterpret_cast<char *>(c.out + token * c.out_stride + (int64_t)qh * c.D);
+            if (!live) dst = nullptr;
+#pragma unroll 1
+            for (int w = 0; w < DB * 2 && have; w++) {
                 uint32_t v[32];
-                __syncwarp();
-                if (have) {
-                    tmem_ld32(v, to + 32 * w);
-                    tmem_wait_ld();
-                }
-                if (two)
+                tmem_ld32(v, to + 32 * w);
+                tmem_wait_ld();
+                if (two) {
 #pragma unroll
                     for (int x = 0; x < 32; x++)
                         v[x] = __float_as_uint(fmaf(a0, __uint_as_float(v[x]), a1 * xo[(32 * w + x) * 128 + trow]));
-                if (live && have && t.part_o) {
-                    float *dst = t.part_o + (blockIdx.z * t.prow + prow) * c.D + 32 * w;
+                }
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4)
-                        if (32 * w + x < c.D)
-                            *reinterpret_cast<uint4 *>(dst + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
-                } else if (live && have) {
-                    uint16_t *dst = c.out + token * c.out_stride + (int64_t)qh * c.D + 32 * w;
+                for (int x = 0; x < 32; x++) v[x] = __float_as_uint(__uint_as_float(v[x]) * inv);
+                __syncwarp();
 #pragma unroll
-                    for (int x = 0; x < 32; x += 8)
-                        if (32 * w + x < c.D) {
-                            uint32_t o[4];
+                for (int x = 0; x < 32; x += 4)
+                    *reinterpret_cast<uint4 *>(stage + lane * 36 + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+                __syncwarp();
+                const int f = 32 * w + (lane & 7) * 4;
 #pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                o[i] = cvt_bf2(__uint_as_float(v[x + 2 * i]) * inv, __uint_as_float(v[x + 2 * i + 1]) * inv);
-                            *reinterpret_cast<uint4 *>(dst + x) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
+                for (int i = 0; i < 8; i++) {
+                    const int r = 4 * i + (lane >> 3);
+                    char *at = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, (unsigned long long)dst, r));
+                    const float4 o = *reinterpret_cast<const float4 *>(stage + r * 36 + (lane & 7) * 4);
+                    if (!at || f >= c.D) continue;
+                    if (t.part_o) *reinterpret_cast<float4 *>(at + f * 4) = o;
+                    else *reinterpret_cast<uint2 *>(at + f * 2) = make_uint2(cvt_bf2(o.x, o.y), cvt_bf2(o.z, o.w));
                 }
             }
         }
