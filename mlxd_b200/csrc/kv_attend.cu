@@ -1069,14 +1069,15 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     }
     L = warp_sum(L);
     const float inv = L > 0.f ? 1.0f / L : 0.f;
+    constexpr int JOIN = 10;                         // loads in flight
     for (int d = lane * 4; d - lane * 4 < c.D; d += 128) {
         const float *po = c.part_o + row * c.D + d;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < c.parts; k += 4) {       // four loads in flight
-            float4 v[4];
-            float a[4];
+        for (int k = 0; k < c.parts; k += JOIN) {
+            float4 v[JOIN];
+            float a[JOIN];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < JOIN; u++) {
                 const float lo = __shfl_sync(0xffffffffu, w[0], (k + u) & 31), hi = __shfl_sync(0xffffffffu, w[1], (k + u) & 31);
                 a[u] = k + u >= c.parts ? 0.f : k + u < 32 ? lo : hi;
                 // a split that saw nothing wrote no row
@@ -1084,7 +1085,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
                                               : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u = 0; u < JOIN; u++) {
                 acc.x = fmaf(a[u], v[u].x, acc.x);
                 acc.y = fmaf(a[u], v[u].y, acc.y);
                 acc.z = fmaf(a[u], v[u].z, acc.z);
