@@ -93,9 +93,9 @@ static float2 *at_ws_ml(void *ws, int D) { return (float2 *)((char *)ws + (size_
 // Up to 16 query rows that share a kv head (the head group of one token, or of
 // a few) against 16 keys a step, on mma.m16n8k16 with the keys and then the
 // features as its 16 rows and the query rows as its 8 columns (the other way
-// round takes twice the MMAs, which at 28 clocks each are the limit here, not
-// HBM: 41 us instead of 29 at one token over 32768 positions). Every key row is
-// read once, in fragment order:
+// round takes up to three times the MMAs, at 28 clocks each: 11.0 against 9.6 us
+// for one token over 2192 positions). Every key row is read once, in fragment
+// order:
 //   scores   S^T = K Q^T: the contraction runs over features, whose order is
 //            free: lane (g, c) = (lane / 4, lane % 4) holds the 16 bytes of
 //            features 32 u + 8 c of keys g and g + 8, the A fragments of two
@@ -152,7 +152,10 @@ __global__ void __launch_bounds__(W * 32)
     auto token_of = [&](int r) { return t.tails ? seq : one ? 0 : (r0 + r) / c.rep; };
     auto qhead_of = [&](int r) { return head * c.rep + (one ? r0 + r : (r0 + r) % c.rep); };
     pdl_trigger();                                 // the kernel that joins may be put in place
-    if (t.tails && c.lens[seq] < 0) return;        // a finished sequence: the whole cluster
+    if (t.tails && c.lens[seq] < 0) {              // a finished sequence: the whole cluster
+        pdl_wait();                                // (no later kernel may overtake the prefix's)
+        return;
+    }
 
     // positions of the rows (lane r: row r; -1: not asked) and the item's keys
     const int rp = lane < nrows ? query_pos(c, token_of(lane)) : -1;
@@ -389,24 +392,26 @@ __global__ void __launch_bounds__(W * 32)
 #pragma unroll
         for (int w = 0; w < W; w++) M = fmaxf(M, sm[w * ROWS + r]);
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (M != -INFINITY)
 #pragma unroll
-            for (int w = 0; w < W; w++) {
-                const float a = ex2((sm[w * ROWS + r] - M) * s2);
-                const float4 v = *reinterpret_cast<const float4 *>(so + (size_t)(w * ROWS + r) * DP + d);
-                acc.x = fmaf(a, v.x, acc.x);
-                acc.y = fmaf(a, v.y, acc.y);
-                acc.z = fmaf(a, v.z, acc.z);
-                acc.w = fmaf(a, v.w, acc.w);
-            }
+        for (int w = 0; w < W; w++) {
+            const float mw = sm[w * ROWS + r], a = mw == -INFINITY ? 0.f : ex2((mw - M) * s2);
+            const float4 v = *reinterpret_cast<const float4 *>(so + (size_t)(w * ROWS + r) * DP + d);
+            acc.x = fmaf(a, v.x, acc.x);
+            acc.y = fmaf(a, v.y, acc.y);
+            acc.z = fmaf(a, v.z, acc.z);
+            acc.w = fmaf(a, v.w, acc.w);
+        }
         *reinterpret_cast<float4 *>(so + (size_t)r * DP + d) = acc;
     }
     __syncthreads();
     if (tid < nrows) {
         float M = -INFINITY, L = 0.f;
         for (int w = 0; w < W; w++) M = fmaxf(M, sm[w * ROWS + tid]);
-        if (M != -INFINITY)
-            for (int w = 0; w < W; w++) L += sl[w * ROWS + tid] * ex2((sm[w * ROWS + tid] - M) * s2);
+        // (a sum that is NaN stays so, whatever its weight)
+        for (int w = 0; w < W; w++) {
+            const float mw = sm[w * ROWS + tid];
+            L = fmaf(sl[w * ROWS + tid], mw == -INFINITY ? 0.f : ex2((mw - M) * s2), L);
+        }
         sm[tid] = M;
         sl[tid] = L;
     }
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(W * 32)
         }
         L = warp_sum(L);
         if (lane == 0) {
-            srow[r] = t.part_o ? 1.f : M == -INFINITY ? 0.f : 1.0f / L;   // a row that sees nothing is zero
+            srow[r] = t.part_o ? 1.f : L == 0.f ? 0.f : 1.0f / L;   // a row that sees nothing is zero
             if (t.part_o && rank % ncl == 0) t.part_ml[blockIdx.x / ncl * t.prow + row] = make_float2(M, L);
         }
     }
@@ -605,7 +610,7 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 //
 //   warp 0, one lane   TMA: key tile j (128 slots x D, 128B swizzle) and value
 //                      tile j into their stages;
-//   warp 1, one lane   per query tile t (two of 128 rows) and key tile j:
+//   warp 1             per query tile t (two of 128 rows) and key tile j:
 //                      S = Q K^T into TMEM, and once the softmax warps have
 //                      put the weights in place of S, O += P V (P from TMEM,
 //                      V as stored: its rows are the contraction);
@@ -616,9 +621,15 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 //                      relative to the maximum in use, so any will do).
 //
 // While one query tile is in its softmax the tensor cores work on the other.
-// Bound by the exponentials (128 x 128 per tile at 16 a clock and SM, 1024
-// clocks) and the tensor cores (2 x 512 clocks) alike when rows are many, by
-// HBM when a prefix is long and the rows are few.
+// Per key tile and 256 rows the MMAs take 2048 clocks and the exponentials as
+// many; the chain S -> maximum -> weights -> P V of a query tile (about 1900 and
+// 900 clocks) leaves 3400. At that rate power sets the clock: a 4096-token chunk
+// at 4096 of 32/8 heads takes 389 us, 1059 TFLOP/s, 75% of the sustained cuBLAS
+// rate (63% of the burst rate); with the softmax left out the same MMAs took
+// 328 us. Tried without gain: exponentials of every 3rd or 4th pair as a cubic on
+// the FMA pipe, a row shared by two threads (500 us: four softmax warps to a
+// scheduler wait for each other's maxima), the MMAs of whichever tile is ready
+// (704 us: both fall into phase).
 // Keys no row of the CTA sees may hold anything: their scores are masked and
 // their value rows zeroed in shared memory. Every wait is bounded; a launch
 // that gave up says so in a host word that the next call reports.
@@ -997,7 +1008,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             const int qh = head * c.rep + row - token * c.rep;
             const int64_t prow = (int64_t)token * c.hq + qh;
             const bool live = p >= 0;
-            const float inv = t.part_o ? 1.f : lsum > 0.f ? 1.0f / lsum : 0.f;
+            const float inv = t.part_o ? 1.f : lsum == 0.f ? 0.f : 1.0f / lsum;
             if (live && t.part_o) t.part_ml[blockIdx.z * t.prow + prow] = make_float2(have ? m : -INFINITY, have ? lsum : 0.f);
             // 32 columns at a time through shared memory (rows of 36 floats, in the value stages), so that 8
             // lanes write one row's
@@ -1068,7 +1079,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
         L = fmaf(w[u], ml[u].y, L);
     }
     L = warp_sum(L);
-    const float inv = L > 0.f ? 1.0f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
     constexpr int JOIN = 10;                         // loads in flight
     for (int d = lane * 4; d - lane * 4 < c.D; d += 128) {
         const float *po = c.part_o + row * c.D + d;

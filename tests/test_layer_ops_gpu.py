@@ -485,6 +485,20 @@ def test_attend_extreme_scores(gen, n):
     c2.check(c2.attend(q, 300, cuda.attn_config(4)), q, 300)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,total", [(1, 100), (1, 9000), (3, 500), (40, 3000), (300, 700)])
+def test_attend_nan_stays_in_its_row(gen, n, total, D):
+    """A query of NaN gives NaN, its neighbours what they would give without it."""
+    c = Cache(gen, 1, D, total, total)
+    q = rand(gen, n, 4, D)
+    clean = c.attend(q, total - n, cuda.attn_config(4))
+    q[n // 2, 2] = math.nan
+    out = c.attend(q, total - n, cuda.attn_config(4))
+    assert bool(out[n // 2, 2].isnan().all())
+    out[n // 2, 2] = clean[n // 2, 2]
+    assert torch.equal(out, clean)
+
+
 def test_attend_other_stream_and_graph(gen):
     """On a stream of its own, and captured once and replayed with new inputs; a second captured call shares the
     workspace in stream order."""
