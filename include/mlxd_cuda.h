@@ -234,9 +234,12 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    attn_workspace_bytes(), 256-byte aligned, that no other call in flight
    uses (calls on one stream may share it). A wrapped ring takes at most
    capacity - cache sinks - window + 1 queries a call, and no more sinks than
-   the cache keeps. Softmax weights are rounded to bf16 for the tensor cores
-   (values times unrounded statistics of the rounded weights); a non-finite
-   value row that one query sees may reach other queries of the same call. */
+   the cache keeps. Scores, softmax statistics and sums are f32; the weights
+   enter the value product rounded to bf16 (with at most 8 query rows per kv
+   head, a token's usual group, as two bf16 terms). A non-finite value row
+   that one query sees may reach other queries of the same call; a NaN query
+   stays alone. Every wait inside is bounded: a launch that gave up makes the
+   next call on any cache fail once. */
 typedef struct {
     int   n_heads;             /* query heads, a multiple of the cache's kv heads */
     int   window;              /* > 0: keys within the last `window` positions */

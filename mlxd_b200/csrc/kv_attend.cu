@@ -1359,7 +1359,7 @@ size_t mlxd_cuda_attn_workspace_bytes(int head_dim) {
 }
 
 int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_stride, int n, int pos,
-                        const mlxd_attn *a, void *out, int64_t out_stride, void *ws, size_t ws_bytes, void *stream) {
+                        const mlxd_attn *a, void *out, int64_t out_stride, void *ws, size_t ws_bytes, void *stream) try {
     if (!kv || layer < 0 || layer >= kv->layers || n < 0 || pos < 0 || (int64_t)pos + n > INT32_MAX) {
         set_error("kv_attend: bad arguments");
         return -1;
@@ -1393,10 +1393,13 @@ int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_s
     c.pos0 = pos;
     c.total = total;
     return attend_cache(c, kv, layer, ws, (cudaStream_t)stream);
+} catch (...) {   // no exception leaves a C entry
+    set_error("kv_attend: out of host memory");
+    return -1;
 }
 
 int mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int prefix_len, int n_seqs,
-                              int tail_capacity) {
+                              int tail_capacity) try {
     if (!out || !prefix || prefix_len < 0 || prefix_len > prefix->cap || n_seqs <= 0 || tail_capacity <= 0 ||
         (int64_t)prefix_len + tail_capacity > INT32_MAX || prefix->d % 8 || prefix->d > 256) {
         set_error("kv_group_create: bad arguments");
@@ -1423,6 +1426,9 @@ int mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int pr
     }
     *out = g;
     return 0;
+} catch (...) {   // no exception leaves a C entry
+    set_error("kv_group_create: out of host memory");
+    return -1;
 }
 
 void mlxd_cuda_kv_group_destroy(mlxd_kv_group *g) {
@@ -1476,7 +1482,7 @@ int mlxd_cuda_kv_group_append(mlxd_kv_group *g, int layer, const void *k, int64_
 
 int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, int64_t q_stride,
                               const int32_t *lens_dev, const mlxd_attn *a, void *out, int64_t out_stride, void *ws,
-                              size_t ws_bytes, void *stream) {
+                              size_t ws_bytes, void *stream) try {
     if (!g || layer < 0 || layer >= g->layers) {
         set_error("kv_group_attend: bad arguments");
         return -1;
@@ -1497,6 +1503,9 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     c.tcap = g->cap;
     c.prefix = c.total = g->prefix_len;
     return attend_group(c, g->prefix, layer, ws, (cudaStream_t)stream);
+} catch (...) {   // no exception leaves a C entry
+    set_error("kv_group_attend: out of host memory");
+    return -1;
 }
 
 }  // extern "C"

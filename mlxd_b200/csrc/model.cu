@@ -934,7 +934,7 @@ int mlxd_cuda_kv_create(mlxd_kv **out, const mlxd_model *m, int capacity) {
 }
 
 int mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int head_dim, int capacity, int window,
-                              int sinks) {
+                              int sinks) try {
     if (!out || layers <= 0 || n_kv_heads <= 0 || head_dim <= 0 || head_dim > 256 || head_dim % 8 || capacity <= 0 ||
         window < 0 || sinks < 0) {
         set_error("kv_create_shape: bad arguments (head_dim: a multiple of 8 up to 256)");
@@ -970,6 +970,9 @@ int mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int hea
     kv_attend_prepare(kv);
     *out = kv;
     return 0;
+} catch (...) {   // no exception leaves a C entry
+    set_error("kv_create_shape: out of host memory");
+    return -1;
 }
 
 void mlxd_cuda_kv_destroy(mlxd_kv *kv) {

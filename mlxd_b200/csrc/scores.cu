@@ -554,7 +554,7 @@ using namespace mlxd;
 
 extern "C" int mlxd_cuda_token_scores(const void *logits, int dtype, int rows, int V, int64_t row_stride,
                                       const int32_t *targets, int n_top, float *logprobs, float *entropy,
-                                      int32_t *top_ids, float *top_logprobs, void *stream) {
+                                      int32_t *top_ids, float *top_logprobs, void *stream) try {
     if ((dtype != MLXD_BF16 && dtype != MLXD_F32) || rows < 0 || V <= 0 || row_stride < 0 || n_top < 0 ||
         n_top > SC_TOP || n_top > V) {
         set_error("token_scores: bad arguments (n_top: at most 32 and V)");
@@ -575,4 +575,7 @@ extern "C" int mlxd_cuda_token_scores(const void *logits, int dtype, int rows, i
     const ScoreCall c = {logits, row_stride, rows, V, n_top, targets, logprobs, entropy, top_logprobs, top_ids};
     return dtype == MLXD_BF16 ? launch_scores<uint16_t>(c, (cudaStream_t)stream)
                               : launch_scores<float>(c, (cudaStream_t)stream);
+} catch (...) {   // no exception leaves a C entry
+    set_error("token_scores: out of host memory");
+    return -1;
 }
