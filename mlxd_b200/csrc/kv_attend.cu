@@ -122,7 +122,7 @@ struct FewCall {
 };
 
 // shared memory of a warp: its ring, later its results
-constexpr int FR_DEPTH = 3;
+constexpr int FR_DEPTH = 2;
 __host__ __device__ constexpr int fr_warp_floats(int nu, int rows) {
     const int nw = (nu + 1) / 2, ring = FR_DEPTH * (2 * nu + 4 * nw) * 32 * 4, res = rows * nw * 64;
     return ring > res ? ring : res;
@@ -480,17 +480,18 @@ __global__ void __launch_bounds__(W * 32)
                     if (k + u < ncl) add(v[u], k + u);
             }
         }
+        constexpr int PF = 10;                       // splits' loads in flight
         const float *po = c.part_o + row * c.D + d;
-        for (int k = 0; k < c.parts; k += 6) {
-            float4 v[6];
+        for (int k = 0; k < c.parts; k += PF) {
+            float4 v[PF];
 #pragma unroll
-            for (int u = 0; u < 6; u++) {
+            for (int u = 0; u < PF; u++) {
                 // a split that saw nothing wrote no row
                 const bool live = k + u < c.parts && sw[(ncl + k + u) * ROWS + r] != 0.f;
                 v[u] = live ? *reinterpret_cast<const float4 *>(po + (k + u) * prow * c.D) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
-            for (int u = 0; u < 6; u++)
+            for (int u = 0; u < PF; u++)
                 if (k + u < c.parts) add(v[u], ncl + k + u);
         }
         if (t.part_o) {
