@@ -13,6 +13,7 @@ f32 accumulation adds 2^-14 for up to 2^10 sequential terms. Scores: sums of
 at most V/128 + 64 sequential f32 terms, each off by 2^-21 of itself."""
 import ctypes as C
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -132,6 +133,36 @@ def test_rope_strides_and_alignment(gen, dtype, off, pad, inter):
     rope_call(x, c, pos, y)
     rope_check(y, x, c, pos)
     assert bool((out[:, :, D:] == 3).all())
+
+
+@pytest.mark.parametrize("n,heads,D,dims,off", [(2368, 70, 256, 32, 1), (2400, 72, 256, 0, 1), (600, 300, 256, 16, 1),
+                                                (1200, 1100, 64, 64, 1), (1184, 33000, 8, 0, 0)])
+def test_rope_many_heads_and_tokens(gen, n, heads, D, dims, off):
+    """More (token, head, feature) items than one CTA takes of several tokens."""
+    x = rand(gen, n * heads * D + off)[off:].view(n, heads, D)
+    y = torch.full((n + 2, heads, D), 3.0, device="cuda", dtype=x.dtype)
+    pos = torch.arange(5, 5 + n, device="cuda", dtype=torch.int32)
+    c = cuda.rope_config(1e4, dims)
+    rope_call(x, c, pos, y[1:-1])
+    for i in range(0, n, 400):
+        rope_check(y[1 + i:1 + min(i + 400, n)], x[i:i + 400], c, pos[i:i + 400])
+    assert bool((y[0] == 3).all()) and bool((y[-1] == 3).all())
+
+
+def test_rope_from_a_thread_without_a_context(gen):
+    """The first CUDA call of a thread."""
+    x = rand(gen, 9, 4, 64)
+    y, c = torch.empty_like(x), cuda.rope_config(1e4, 64)
+    pos = torch.arange(9, device="cuda", dtype=torch.int32)
+    torch.cuda.synchronize()
+    args = (x.data_ptr(), cuda.BF16, 9, 4, 64, 256, 64, C.byref(c), pos.data_ptr(), 0, y.data_ptr(), 256, 64, None)
+    rc = []
+    t = threading.Thread(target=lambda: rc.append(cuda.lib().mlxd_cuda_rope(*args)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert rc == [0]
+    rope_check(y, x, c, pos)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
