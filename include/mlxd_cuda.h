@@ -313,7 +313,8 @@ int mlxd_cuda_sample(const void *logits_dev, int dtype, int V, const mlxd_sampli
    may be NULL when logprobs is. -inf logits have probability zero; a row
    without any other is an empty distribution: logprobs -inf, entropy 0, top
    ids in index order. A row with +inf or NaN gives NaN scores (its ids order
-   NaN last). A target outside the row gives NaN. */
+   NaN last). A target outside the row gives NaN.
+   Repeated calls give the same bits. */
 int mlxd_cuda_token_scores(const void *logits_dev, int dtype, int rows, int V, int64_t row_stride,
                            const int32_t *targets_dev, int n_top, float *logprobs_dev, float *entropy_dev,
                            int32_t *top_ids_dev, float *top_logprobs_dev, void *stream);

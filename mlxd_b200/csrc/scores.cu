@@ -11,12 +11,13 @@
 // logits, bounds its k-th largest logit from below. A logit that reaches T goes
 // to a list in shared memory (for random orders some 4 k of them); all others
 // are summed relative to the first part's maximum, which they cannot exceed. At
-// the end the listed logits but the largest join the sums (so a peaked row
-// keeps its small terms), and the list is ranked by counting; keys (value,
-// index) are distinct, ties cost nothing. A logit that finds the list full is
-// kept out of its thread's sums while it is its largest, and the list is made
-// again from the whole row's group maxima. Measured, 512 rows of 151936 bf16 with 20
-// alternatives: 50 us, 47% of the measured copy rate; 37 of them without the
+// the end the list is ranked by counting (keys of value and index are distinct,
+// ties cost nothing), and the listed logits but the largest join the sums in that
+// order (a peaked row keeps its small terms; the threads' timing changes no bit).
+// A row whose list overflows (rising or strided rows, thousands of ties) is read
+// again with every thread's largest logit held out of its sums, and the list is
+// made from the whole row's group maxima. Measured, 512 rows of 151936 bf16 with
+// 20 alternatives: 50 us, 48% of the measured copy rate; 37 of them without the
 // sums, the rest of the distance the selection's serial steps at a row's end.
 #include "common.cuh"
 #include "kernels.h"
@@ -188,7 +189,7 @@ template <typename T>
 __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_constant__ ScoreCall c) {
     constexpr int N = 16 / sizeof(T), NWARP = SC_THREADS / 32;
     __shared__ ScorePart part;
-    __shared__ u64 s_wkey[NWARP], s_gkey[SC_GROUPS], s_cand[SC_CAND], s_t;
+    __shared__ u64 s_wkey[NWARP], s_gkey[SC_GROUPS], s_cand[SC_CAND], s_sort[SC_CAND], s_t;
     __shared__ float s_ws[NWARP][2];
     __shared__ int s_flag[SC_THREADS], s_nflag, s_ncand;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -311,22 +312,16 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
 #pragma unroll
             for (int j = 0; j < M; j++) hit |= e[j] >= tv ? 1u << j : 0u;
             int at = atomicAdd(&s_ncand, __popc(hit));
-            if (at + __popc(hit) <= SC_CAND) {
+            if (at + __popc(hit) > SC_CAND) return;  // the row is summed again
 #pragma unroll
-                for (int j = 0; j < M; j++)
-                    if (hit >> j & 1) {
-                        s_cand[at++] = sc_key(e[j], base + j);
-                        e[j] = -INFINITY;
-                    }
-            } else {
-                for (; at < SC_CAND; at++) s_cand[at] = 0ull;   // reserved, left empty
-                sc_add<M>(a, e, base);
-                return;
-            }
+            for (int j = 0; j < M; j++)
+                if (hit >> j & 1) {
+                    s_cand[at++] = sc_key(e[j], base + j);
+                    e[j] = -INFINITY;
+                }
         }
         sc_sum<M>(a, e);
     };
-    // in index order: a thread holds out the first of equal logits
     if (tid < min(head, extras)) {
         float e[1] = {sc_load(x, tid)};
         add(e, e[0] >= tv, tid);
@@ -349,19 +344,52 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
         add(e, e[0] >= tv, extra_at(tid));
     }
     __syncthreads();
-    const int nc = s_ncand, listed = min(nc, SC_CAND);
 
-    // the CTA's largest logit and the sums of the rest
-    const u64 mine = a.best > -INFINITY ? sc_key(a.best, a.at) : 0ull;
-    u64 key = mine;
-    for (int i = tid; i < listed; i += SC_THREADS) key = s_cand[i] > key ? s_cand[i] : key;
-    key = block_max64(key);
-    if (key) {
-        const float m = sc_val(key);
-        sc_move(a.s, a.w, a.ref, m);
-        if (mine && mine != key) sc_join(a.s, a.w, a.best, m);
-        for (int i = tid; i < listed; i += SC_THREADS)
-            if (s_cand[i] && s_cand[i] != key) sc_join(a.s, a.w, sc_val(s_cand[i]), m);
+    // The CTA's largest logit and the sums of the rest. The list's order depends
+    // on the threads' timing, its ranks do not: they give the same bits every time.
+    int n = s_ncand;
+    auto sort = [&] {
+        ranks(s_cand, n, [&](u64 k, int above) { s_sort[above] = k; });
+        __syncthreads();
+    };
+    u64 key = 0;
+    if (n <= SC_CAND) {
+        sort();
+        if (n) {
+            key = s_sort[0];
+            const float m = sc_val(key);
+            sc_move(a.s, a.w, a.ref, m);
+            for (int i = tid ? tid : SC_THREADS; i < n; i += SC_THREADS) sc_join(a.s, a.w, sc_val(s_sort[i]), m);
+        }
+    } else {
+        // again, in index order (a thread holds out the first of equal logits), and the list from these maxima
+        a.s = a.w = 0.f;
+        if (tid < min(head, extras)) {
+            float e[1] = {sc_load(x, tid)};
+            sc_add<1>(a, e, tid);
+        }
+        for (int v = v0 + tid; v < v1; v += SC_THREADS) {
+            float e[N];
+            sc_unpack(ldg_nc_v4(xv + v), e);
+            sc_add<N>(a, e, head + v * N);
+        }
+        if (tid >= head && tid < extras) {
+            float e[1] = {sc_load(x, extra_at(tid))};
+            sc_add<1>(a, e, extra_at(tid));
+        }
+        const u64 mine = a.best > -INFINITY ? sc_key(a.best, a.at) : 0ull;
+        key = block_max64(mine);
+        if (key) {
+            const float m = sc_val(key);
+            sc_move(a.s, a.w, a.ref, m);
+            if (mine && mine != key) sc_join(a.s, a.w, a.best, m);
+        }
+        if (c.top) {
+            if (tid == 0) s_ncand = 0;
+            collect(mine);
+            n = s_ncand;
+            if (n <= SC_CAND) sort();
+        }
     }
     a.s = warp_sum(a.s);
     a.w = warp_sum(a.w);
@@ -381,32 +409,20 @@ __global__ void __launch_bounds__(SC_THREADS, 4) scores_kernel(const __grid_cons
         part.w = w;
     }
     if (c.top) {
-        int n = nc;
-        // every logit above -inf of this CTA, as a key, to f
-        auto each = [&](auto f) {
-            if (tid < extras) f(sc_load(x, extra_at(tid)), extra_at(tid));
-            for (int v = v0 + tid; v < v1; v += SC_THREADS) {
-                float e[N];
-                sc_unpack(ldg_nc_v4(xv + v), e);
-#pragma unroll
-                for (int j = 0; j < N; j++) f(e[j], head + v * N + j);
-            }
-        };
-        if (n > SC_CAND) {                           // again, with the whole row's group maxima
-            u64 b = 0;
-            each([&](float v, int i) {
-                if (v > -INFINITY) b = max(b, sc_key(v, i));
-            });
-            if (tid == 0) s_ncand = 0;
-            collect(b);
-            n = s_ncand;
-        }
         if (n <= SC_CAND) {
-            ranks(s_cand, n, [&](u64 k, int above) {
-                if (above < c.top) part.list[above] = k;
-            });
+            if (tid < min(n, c.top)) part.list[tid] = s_sort[tid];
             if (tid == 0) part.count = min(n, c.top);
         } else {
+            // every logit above -inf of this CTA, as a key, to f
+            auto each = [&](auto f) {
+                if (tid < extras) f(sc_load(x, extra_at(tid)), extra_at(tid));
+                for (int v = v0 + tid; v < v1; v += SC_THREADS) {
+                    float e[N];
+                    sc_unpack(ldg_nc_v4(xv + v), e);
+#pragma unroll
+                    for (int j = 0; j < N; j++) f(e[j], head + v * N + j);
+                }
+            };
             // a few threads hold nearly all of the largest: the largest below the last one, again and again
             u64 last = ~0ull;
             for (int r = 0; r < c.top; r++) {

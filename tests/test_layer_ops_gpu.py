@@ -319,6 +319,27 @@ def test_scores_rows_ordered_against_the_scan(gen, kind, rows, dtype):
     scores_check(scores_call(x, t, 20), x, t, 20)
 
 
+@pytest.mark.parametrize("kind", ["random", "rising", "ties", "strided"])
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_scores_repeat_bit_for_bit(gen, kind, rows):
+    """Whatever order the threads meet the largest logits in (and when they are too many to list)."""
+    V = 60013
+    x = rand(gen, rows, V, dtype=torch.float32, scale=3.0)
+    at = torch.arange(V, device="cuda")
+    if kind == "rising":
+        x += at * 1e-3
+    elif kind == "ties":
+        x = torch.round(x)
+    elif kind == "strided":
+        x[:, (at // 4) % 256 < 3] += 9.0
+    t = torch.randint(0, V, (rows,), device="cuda", generator=gen).to(torch.int32)
+    first = scores_call(x, t, 20)
+    for _ in range(20):
+        again = scores_call(x, t, 20)
+        for k in first:
+            assert torch.equal(again[k], first[k]), k
+
+
 def test_scores_peaked_rows_keep_their_small_terms(gen):
     """A row whose other tokens hold 1e-12 of the mass: entropy and logprob to f32 precision of themselves."""
     V = 3001
