@@ -456,6 +456,16 @@ class Model:
             pass
 
 
+def row_count(k, v, shape):
+    """n of device arrays k and v, which must be contiguous [Hkv][n][D] of 2-byte elements (the
+    library sees their addresses alone)."""
+    hkv, D = shape
+    for a in (k, v):
+        if (tuple(a.shape) != (hkv, k.shape[1], D) or not a.is_contiguous() or a.element_size() != 2):
+            raise ValueError("cache rows: contiguous bf16 arrays [%d][n][%d], the same n for k and v" % (hkv, D))
+    return k.shape[1]
+
+
 class KVCache:
     """kvcache_t over libmlxd_cuda (src/engine/kvcache.h:11-51)."""
 
@@ -478,8 +488,15 @@ class KVCache:
 
     def write(self, layer, pos, k, v, stream=None):
         """kvcache_update: rows [pos, pos + n) from device arrays k, v [Hkv][n][D] (tensors)."""
-        check(lib().mlxd_cuda_kv_write(self.kv, layer, pos, k.shape[1], dev_ptr(k), dev_ptr(v), stream),
-              "kv_write")
+        n = row_count(k, v, self.row_shape())
+        check(lib().mlxd_cuda_kv_write(self.kv, layer, pos, n, dev_ptr(k), dev_ptr(v), stream), "kv_write")
+
+    def row_shape(self):
+        """(kv heads, head dim) of a cached position."""
+        if self.model is None:
+            return self.shape
+        c = self.model.cfg
+        return c.n_kv_heads // max(c.tp_size, 1), c.head_dim
 
     def offset(self, layer=0):
         return lib().mlxd_cuda_kv_offset(self.kv, layer)
@@ -491,11 +508,7 @@ class KVCache:
         check(lib().mlxd_cuda_kv_reset(self.kv), "kv_reset")
 
     def read(self, layer, value=False):
-        if self.model is None:
-            hkv, head_dim = self.shape
-        else:
-            c = self.model.cfg
-            hkv, head_dim = c.n_kv_heads // max(c.tp_size, 1), c.head_dim
+        hkv, head_dim = self.row_shape()
         cap = self.capacity(layer)
         buf = np.zeros((hkv, cap, head_dim), dtype=np.uint16)
         n = C.c_int()
@@ -527,8 +540,9 @@ class KVGroup:
 
     def write(self, layer, seq, row, k, v, stream=None):
         """Tail rows [row, row + n) of one sequence from device arrays k, v [Hkv][n][D] (tensors)."""
-        check(lib().mlxd_cuda_kv_group_write(self.g, layer, seq, row, k.shape[1], dev_ptr(k), dev_ptr(v),
-                                             stream), "kv_group_write")
+        n = row_count(k, v, self.prefix.row_shape())
+        check(lib().mlxd_cuda_kv_group_write(self.g, layer, seq, row, n, dev_ptr(k), dev_ptr(v), stream),
+              "kv_group_write")
 
     def close(self):
         if getattr(self, "g", None):
@@ -634,8 +648,11 @@ def rope(x, cfg, pos):
     dt = BF16 if x.dtype == np.uint16 else F32
     if dt == F32:
         x = x.astype(np.float32, copy=False)
+    pos = np.asarray(pos, np.int32)
+    if pos.shape not in ((), (n,)):
+        raise ValueError("rope: %s positions for %d tokens" % (pos.shape, n))
     dx, dy = DeviceBuffer.from_array(x), DeviceBuffer(x.nbytes)
-    per = None if np.isscalar(pos) else DeviceBuffer.from_array(np.asarray(pos, np.int32))
+    per = DeviceBuffer.from_array(pos) if pos.ndim else None
     check(lib().mlxd_cuda_rope(dx.ptr, dt, n, heads, D, heads * D, D, C.byref(cfg),
                                per.ptr if per else None, 0 if per else int(pos), dy.ptr, heads * D, D, None),
           "rope")
@@ -650,7 +667,10 @@ def token_scores(logits, targets, n_top=0):
     dt = BF16 if x.dtype == np.uint16 else F32
     if dt == F32:
         x = x.astype(np.float32, copy=False)
-    dx, dt_ids = DeviceBuffer.from_array(x), DeviceBuffer.from_array(np.asarray(targets, np.int32))
+    targets = np.asarray(targets, np.int32)
+    if targets.shape != (rows,):
+        raise ValueError("token_scores: %s targets for %d rows" % (targets.shape, rows))
+    dx, dt_ids = DeviceBuffer.from_array(x), DeviceBuffer.from_array(targets)
     lp, ent = DeviceBuffer(rows * 4), DeviceBuffer(rows * 4)
     ids, tlp = DeviceBuffer(rows * n_top * 4), DeviceBuffer(rows * n_top * 4)
     check(lib().mlxd_cuda_token_scores(dx.ptr, dt, rows, V, V, dt_ids.ptr, n_top, lp.ptr, ent.ptr, ids.ptr,

@@ -5,6 +5,7 @@ import ctypes as C
 
 import numpy as np
 import pytest
+import torch
 
 from mlxd_b200 import cuda
 
@@ -105,3 +106,28 @@ def test_workspace_size_is_known_without_a_device():
     assert cuda.attn_workspace_bytes(128) > 0
     assert cuda.attn_workspace_bytes(128) >= cuda.attn_workspace_bytes(64)
     assert cuda.attn_workspace_bytes(0) == 0
+
+
+def test_host_wrappers_refuse_lengths_that_do_not_match():
+    x = np.zeros((3, 2, 8), np.float32)
+    for pos in (np.arange(2), np.arange(4), np.zeros((3, 1))):
+        with pytest.raises(ValueError, match="positions for 3 tokens"):
+            cuda.rope(x, cuda.rope_config(1e4, 8), pos)
+    for targets in ([1, 2], [1, 2, 3, 4], 1):
+        with pytest.raises(ValueError, match="targets for 3 rows"):
+            cuda.token_scores(np.zeros((3, 16), np.float32), targets)
+
+
+@pytest.mark.parametrize("k,v", [((2, 5, 16), (2, 4, 16)), ((2, 5, 16), (1, 5, 16)), ((3, 5, 16), (3, 5, 16)),
+                                 ((2, 5, 8), (2, 5, 8)), ((10, 16), (10, 16))])
+def test_cache_rows_refuse_shapes(k, v):
+    with pytest.raises(ValueError, match="cache rows"):
+        cuda.row_count(torch.zeros(k, dtype=torch.bfloat16), torch.zeros(v, dtype=torch.bfloat16), (2, 16))
+
+
+def test_cache_rows_refuse_strides_and_types():
+    a = torch.zeros(2, 5, 16, dtype=torch.bfloat16)
+    assert cuda.row_count(a, a, (2, 16)) == 5
+    for b in (a.transpose(0, 1).contiguous().transpose(0, 1), a[:, ::2], a.float()):
+        with pytest.raises(ValueError, match="cache rows"):
+            cuda.row_count(b, b, (2, 16))
