@@ -1212,15 +1212,15 @@ static bool row_map(CUtensorMap *m, const uint16_t *base, int heads, int cap, in
 }
 
 void kv_attend_prepare(mlxd_kv *kv) {
-    fail_word(true);
-    kv->maps = kv->d % 8 == 0 && kv->d <= 128 && row_map(&kv->map_k, kv->k, kv->layers * kv->hkv, kv->cap, kv->d) &&
+    // (no tiles without the word that reports their failures)
+    kv->maps = fail_word(true) && kv->d % 8 == 0 && kv->d <= 128 && row_map(&kv->map_k, kv->k, kv->layers * kv->hkv, kv->cap, kv->d) &&
                row_map(&kv->map_v, kv->v, kv->layers * kv->hkv, kv->cap, kv->d);
 }
 
 static int attend_tiles(const AttnCall &c, const mlxd_kv *kv, int layer, TileShape shape, bool partial, void *ws,
                         cudaStream_t st) {
     if (!kv->maps) {
-        set_error("attention: the cache has no tensor maps (driver without cuTensorMapEncodeTiled)");
+        set_error("attention: the cache has no tensor maps (no cuTensorMapEncodeTiled, or no pinned host memory)");
         return -1;
     }
     TileCall t = {};
