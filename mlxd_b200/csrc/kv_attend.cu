@@ -95,7 +95,7 @@ static float2 *at_ws_ml(void *ws, int D) { return (float2 *)((char *)ws + (size_
 // a few) against 16 keys a step, on mma.m16n8k16 with the keys and then the
 // features as its 16 rows and the query rows as its 8 columns (the other way
 // round takes up to three times the MMAs, at 28 clocks each: 11.0 against 9.6 us
-// for one token over 2192 positions). Every key row is read once, in fragment
+// for one token over 2192 positions). Every key row is read once; in fragment
 // order:
 //   scores   S^T = K Q^T: the contraction runs over features, whose order is
 //            free: lane (g, c) = (lane / 4, lane % 4) holds the 16 bytes of
@@ -179,35 +179,40 @@ __global__ void __launch_bounds__(W * 32)
         kb = c.k + (size_t)head * c.cap * c.D;
         vb = c.v + (size_t)head * c.cap * c.D;
     }
+    // (consecutive runs lie on different CTAs, so the longer ones do too)
     const int na = (sp.a1 + 15) / 16, nc = (max(0, sp.c1 - sp.c0) + 15) / 16, nb = (max(0, sp.b1 - sp.b0) + 15) / 16;
-    const int ns = na + nc + nb, wg = rank * W + warp, nwg = ncta * W;
-    const int st0 = (int)((int64_t)ns * wg / nwg), st1 = (int)((int64_t)ns * (wg + 1) / nwg);
+    const int ns = na + nc + nb, wg = warp * ncta + rank, nwg = ncta * W;
+    const int each = ns / nwg, more = ns - each * nwg;   // the first `more` warps take one step more
+    const int st0 = each * wg + min(wg, more), st1 = st0 + each + (wg < more);
 
     auto step_slots = [&](int st, int &s, int &e) {
         const bool a = st < na, b = st >= na + nc;
         s = a ? 16 * st : b ? sp.b0 + 16 * (st - na - nc) : sp.c0 + 16 * (st - na);
         e = a ? sp.a1 : b ? sp.b1 : sp.c1;
     };
-    // A step's rows go through a ring of FR_DEPTH stages in shared memory in which every lane reads back what
-    // it copied itself: deep prefetch without registers, layouts or barriers.
+    // A step's rows go through a ring of FR_DEPTH stages in shared memory, the warp's own: deep prefetch without
+    // registers or CTA barriers.
     constexpr int KV = 2 * NU + 4 * NW;              // 16-byte pieces of a lane per step
     uint4 *ring = reinterpret_cast<uint4 *>(fsm) + (size_t)warp * FR_DEPTH * KV * 32 + lane;
     int put = 0, get = 0;                            // ring stages
+    // The keys' pieces [16][4 NU] are copied in whole rows, so that an instruction meets 4 cache lines and not 8 (what
+    // bounds the copies is the rate of lines: 131072 positions 115 -> 105 us, 32768 35.5 -> 33.4); odd rows swap
+    // their 64-byte halves where two rows would start at one bank. Each lane copies the values' pieces that it reads.
+    constexpr int CH = 4 * NU;
+    auto key_at = [&](int row, int chunk) { return row * CH + (NU % 2 ? chunk : chunk ^ (row & 1) << 2); };
+    uint4 *kring = ring - lane;
     auto fetch = [&](int ahead) {
         if (ahead < st1) {
             int s, e;
             step_slots(ahead, s, e);
-            uint4 *dst = ring + put * KV * 32;
+            uint4 *dst = ring + put * KV * 32, *kdst = kring + put * KV * 32;
             put = put + 1 == FR_DEPTH ? 0 : put + 1;
             // past the end: the last row again, its score masked; past D: zeros
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint16_t *row = kb + (size_t)min(s + 8 * i + g, e - 1) * c.D + 8 * cc;
-#pragma unroll
-                for (int u = 0; u < NU; u++) {
-                    const bool in = 32 * u + 8 * cc < c.D;
-                    cp_async16_zfill(dst + (2 * u + i) * 32, in ? row + 32 * u : kb, in);
-                }
+            for (int i = 0; i < 2 * NU; i++) {
+                const int at = 32 * i + lane, row = at / CH, chunk = at % CH;
+                const bool in = 8 * chunk < c.D;
+                cp_async16_zfill(kdst + key_at(row, chunk), in ? kb + (size_t)min(s + row, e - 1) * c.D + 8 * chunk : kb, in);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -254,9 +259,11 @@ __global__ void __launch_bounds__(W * 32)
 
 #pragma unroll 1
     for (int st = st0; st < st1; st++) {
+        __syncwarp();                                // the stage has been read
         fetch(st + FR_DEPTH - 1);
         cp_async_wait<FR_DEPTH - 1>();
-        const uint4 *src = ring + get * KV * 32;
+        __syncwarp();
+        const uint4 *src = ring + get * KV * 32, *ks = kring + get * KV * 32;
         get = get + 1 == FR_DEPTH ? 0 : get + 1;
         // scores of keys g and g + 8 (rows) in this lane's columns, as two chains
         float z[NT][4], z1[NT][4];
@@ -266,7 +273,7 @@ __global__ void __launch_bounds__(W * 32)
             for (int x = 0; x < 4; x++) z[i][x] = z1[i][x] = 0.f;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
-            const uint4 k0 = src[2 * u * 32], k1 = src[(2 * u + 1) * 32];
+            const uint4 k0 = ks[key_at(g, 4 * u + cc)], k1 = ks[key_at(g + 8, 4 * u + cc)];
             const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
 #pragma unroll
             for (int i = 0; i < NT; i++) {
@@ -575,9 +582,10 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
     }
     FewCall t = {};
     t.tails = kind == FEW_TAILS;
-    // CTAs per item: as many as fill the SMs while each of their warps has two steps of 16 keys
-    const int W = c.D > 128 || items >= num_sms() ? 4 : 8;   // items enough: two CTAs to an SM
-    int64_t s = num_sms() / items;
+    // CTAs per item: as many as fill the SMs (items enough: three CTAs of 4 warps to an SM; 24 sequences of up to
+    // 4096 own tokens 91 us, against 145 with one) while each of their warps has two steps of 16 keys
+    const int W = c.D > 128 || items >= num_sms() ? 4 : 8;
+    int64_t s = (W == 4 && c.D <= 128 ? 3 : 1) * num_sms() / items;
     if (s > (keys + W * 32 - 1) / (W * 32)) s = (keys + W * 32 - 1) / (W * 32);
     if (s > FR_PARTS) s = FR_PARTS;
     if (s > AT_WS_ROWS / qrows) s = AT_WS_ROWS / qrows;
