@@ -634,14 +634,16 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 //
 // While one query tile is in its softmax the tensor cores work on the other.
 // Per key tile and 256 rows the MMAs take 2048 clocks and the exponentials as
-// many; the chain S -> maximum -> weights -> P V of a query tile (about 1900 and
-// 900 clocks) leaves 3400. At that rate power sets the clock: a 4096-token chunk
-// at 4096 of 32/8 heads takes 389 us, 1059 TFLOP/s, 75% of the sustained cuBLAS
-// rate (63% of the burst rate); with the softmax left out the same MMAs took
-// 328 us. Tried without gain: exponentials of every 3rd or 4th pair as a cubic on
-// the FMA pipe, a row shared by two threads (500 us: four softmax warps to a
-// scheduler wait for each other's maxima), the MMAs of whichever tile is ready
-// (704 us: both fall into phase).
+// many; the chain S -> maximum -> weights -> P V -> S of a query tile leaves some
+// 3700 (tensor pipe and exponentials 56% busy). A 4096-token chunk at 4096 of
+// 32/8 heads takes 380 us, 1084 TFLOP/s, 64% of the cuBLAS burst rate, at the
+// power limit (1.7 GHz); with the softmax left out the same MMAs took 328 us. The
+// first weights are taken by the old maximum while the new one is found, and
+// again when it grew (398 -> 384 us). Tried without gain: exponentials of every
+// 3rd or 4th pair as a cubic on the FMA pipe, a row shared by two threads (500
+// us: four softmax warps to a scheduler wait for each other's maxima), the MMAs
+// of whichever tile is ready (704 us: both fall into phase), weights stored 32
+// keys at a time (402 us), three key or value stages.
 // Keys no row of the CTA sees may hold anything: their scores are masked and
 // their value rows zeroed in shared memory. Every wait is bounded; a launch
 // that gave up says so in a host word that the next call reports.
@@ -687,8 +689,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     __shared__ int s_min[8], s_max[8], s_fail;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int head = blockIdx.y, rows = c.n * c.rep;
-    const int r0 = (gridDim.x - 1 - blockIdx.x) * (BK ? 128 : AT_ROWS);   // the longest rows first
+    // Several waves: the longest rows of all heads first (a head after another: 4096-token chunk 385 us, against
+    // 380). One wave: a head's tiles side by side, which share its keys' way to the SMs.
+    const int rows = c.n * c.rep, head = BK ? blockIdx.y : blockIdx.x;
+    const int r0 = BK ? (gridDim.x - 1 - blockIdx.x) * 128 : (gridDim.y - 1 - blockIdx.y) * AT_ROWS;
     const int nq = BK || rows - r0 > 128 ? 2 : 1;
     if (tid == 0) {
         for (int i = 0; i < 2 * (KS + VS); i++) mbar_init(&kfull[i], 1);
@@ -1147,9 +1151,9 @@ static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &
                        cudaStream_t st) {
     auto kern = attend_tile_kernel<DB, BK>;
     if (!smem_allowed((const void *)kern, (AtLayout<DB, BK>::TOTAL))) return -1;
-    const int per = BK ? 128 : AT_ROWS;
-    const int64_t blocks = ((int64_t)c.n * c.rep + per - 1) / per;
-    kern<<<dim3((unsigned)blocks, c.hkv, t.splits), AT_THREADS, (AtLayout<DB, BK>::TOTAL), st>>>(mk, mv, c, t);
+    const int per = BK ? 128 : AT_ROWS, blocks = (c.n * c.rep + per - 1) / per;
+    const dim3 grid(BK ? blocks : c.hkv, BK ? c.hkv : blocks, t.splits);
+    kern<<<grid, AT_THREADS, (AtLayout<DB, BK>::TOTAL), st>>>(mk, mv, c, t);
     MLXD_CHECK(cudaGetLastError());
     return 0;
 }
@@ -1157,7 +1161,8 @@ static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &
 // The shape of a tile launch. A CTA of 128 rows whose halves alternate key
 // tiles takes about half the time of one of 256 rows whose halves share every
 // key tile. While the former fit one wave they are taken (a 512-token chunk
-// over a 4096 window 60 us, against 69 in 256 rows and two splits), beyond it
+// over a 4096 window 60 us, against 69 in 256 rows and two splits, when this
+// was chosen; 51 now), beyond it
 // the latter, with half the loads per product (a 4096-token chunk 415 us, against
 // 514). Key splits fill the SMs when even those are few, no more than the key
 // tiles or the workspace's rows.
@@ -1262,7 +1267,7 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
     // more than 8 rows per kv head: tiles (16 rows at 8192 positions 18.4 us, against 21.8 with 16 columns of
     // the few-rows kernel; 8 rows 16.9, against 17.5 on tiles)
     if (c.D <= 128 && rows > 8) {
-        if (rows > INT_MAX - AT_ROWS || c.hkv > 65535) {
+        if (rows > 65535 * AT_ROWS || c.hkv > 65535) {   // the grid's limits
             set_error("kv_attend: too many query rows");
             return -1;
         }
