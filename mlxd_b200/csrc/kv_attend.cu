@@ -636,7 +636,7 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 // Per key tile and 256 rows the MMAs take 2048 clocks and the exponentials as
 // many; the chain S -> maximum -> weights -> P V -> S of a query tile leaves some
 // 3700 (tensor pipe and exponentials 56% busy). A 4096-token chunk at 4096 of
-// 32/8 heads takes 380 us, 1084 TFLOP/s, 64% of the cuBLAS burst rate, at the
+// 32/8 heads takes 379 us, 1087 TFLOP/s, 65% of the cuBLAS burst rate, at the
 // power limit (1.7 GHz); with the softmax left out the same MMAs took 328 us. The
 // first weights are taken by the old maximum while the new one is found, and
 // again when it grew (398 -> 384 us). Tried without gain: exponentials of every
@@ -689,8 +689,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     __shared__ int s_min[8], s_max[8], s_fail;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // Several waves: the longest rows of all heads first (a head after another: 4096-token chunk 385 us, against
-    // 380). One wave: a head's tiles side by side, which share its keys' way to the SMs.
+    // Several waves: the longest rows of all heads first (a head after another: 4096-token chunk 384 us, against
+    // 379). One wave: a head's tiles side by side, which share its keys' way to the SMs.
     const int rows = c.n * c.rep, head = BK ? blockIdx.y : blockIdx.x;
     const int r0 = BK ? (gridDim.x - 1 - blockIdx.x) * 128 : (gridDim.y - 1 - blockIdx.y) * AT_ROWS;
     const int nq = BK || rows - r0 > 128 ? 2 : 1;
