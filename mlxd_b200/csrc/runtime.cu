@@ -69,7 +69,7 @@ bool on_device(const void *p, const char *what, int align) {
         set_error("%s: not aligned to %d bytes", what, align);
         return false;
     }
-    // the driver's query of the three attributes (the runtime's gathers more, at twice the time)
+    // libcuda's query of the three attributes (the runtime's gathers more, at twice the time)
     static const PointerGetAttributesFn get = [] {
         void *f = nullptr;
         cudaDriverEntryPointQueryResult q;
