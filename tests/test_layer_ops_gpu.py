@@ -774,6 +774,41 @@ def test_shared_prefix_many_sequences(gen):
         assert torch.equal(out, t.attend(q, ld, cuda.attn_config(32)))
 
 
+@pytest.mark.parametrize("D,seqs,tail", [(128, 24, 1500), (64, 20, 900), (96, 19, 700)])
+def test_shared_prefix_long_tails(gen, D, seqs, tail):
+    """Items that fill the SMs two or three times over: a cluster to a tail, some of them ended, empty or full."""
+    t = Group(gen, 8, D, 1000, 1100, seqs, tail, layers=1, layer=0)
+    lens = [int(v) for v in torch.randint(1, tail + 1, (seqs,), device="cuda", generator=gen)]
+    lens[0], lens[1], lens[2], lens[3] = 0, -1, tail, 1
+    t.fill(lens)
+    q = rand(gen, seqs, 32, D, scale=1.5)
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = t.attend(q, ld, cuda.attn_config(32))
+    t.check(out, q, lens, seqs=[0, 1, 2, 3, seqs - 1])
+    for _ in range(5):
+        again = t.attend(q, ld, cuda.attn_config(32))
+        keep = [i for i in range(seqs) if lens[i] >= 0]
+        assert torch.equal(out[keep], again[keep])
+
+
+@pytest.mark.parametrize("hkv,D", [(160, 64), (200, 32)])
+def test_attend_single_token_many_kv_heads(gen, hkv, D):
+    c = Cache(gen, hkv, D, 700, 650, layers=1, layer=0)
+    q = rand(gen, 1, hkv, D, scale=1.5)
+    a = c.attend(q, 649, cuda.attn_config(hkv))
+    c.check(a, q, 649, heads=[0, 1, hkv // 2, hkv - 1])
+    assert torch.equal(a, c.attend(q, 649, cuda.attn_config(hkv)))
+
+
+def test_attend_long_chunk_over_heads(gen):
+    """More tiles than one wave, an odd number of them: every head's rows at their places."""
+    c = Cache(gen, 5, 128, 2200, 2190, layers=1, layer=0)
+    q = rand(gen, 1990, 20, 128, scale=1.5)
+    a = c.attend(q, 200, cuda.attn_config(20))
+    c.check(a, q, 200, heads=[0, 3, 4, 11, 19])
+    assert torch.equal(a, c.attend(q, 200, cuda.attn_config(20)))
+
+
 def test_group_decode_loop_in_a_graph(gen):
     """append + attend captured once and replayed with lengths that grow on the device, as a batched decode loop runs
     them; a finished sequence's rows stay."""
