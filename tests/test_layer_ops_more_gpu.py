@@ -1,0 +1,207 @@
+"""Attention over a cache and of a shared prefix where the plain comparison is blind: every key is counted once,
+maxima that rise along the keys, the bf16 pairs of few rows; against 64-bit forms.
+
+Tolerances: a rounding to bf16 is off by at most 2^-8 of the value. Weights rounded to bf16 over the sum of the same
+rounded weights move the normalised weights by at most 2 * 2^-8, weights held as two bf16 terms (8 + 8 bits and a sign)
+by at most 2 * 2^-17. A score of D products in f32 is off by (D + 4) 2^-24 of sum |q k|, and enters exponents twice."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from mlxd_b200 import cuda
+from tests.test_layer_ops_gpu import Cache, Group, attn_row, rand, seen
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    cuda.init(0)
+    yield
+
+
+@pytest.fixture
+def gen():
+    return torch.Generator(device="cuda").manual_seed(77)
+
+
+def put(c, k=None, v=None):
+    """Other rows for every position of a Cache, in runs that fit its ring."""
+    total, ring, a = c.k.shape[1], c.kv.capacity() - c.sinks, 0
+    c.k, c.v = c.k if k is None else k, c.v if v is None else v
+    while a < total:
+        step = min(total - a, c.sinks - a if a < c.sinks else ring)
+        c.kv.write(c.layer, a, c.k[:, a:a + step].contiguous(), c.v[:, a:a + step].contiguous())
+        a += step
+
+
+def cache(g, hkv, D, cap, total, window=0, sinks=0):
+    c = Cache(g, hkv, D, cap, total, window=window, sinks=sinks, layers=1, layer=0)
+    c.sinks = sinks
+    return c
+
+
+# ------------------------------------------------------------------ every key once
+
+def counts(hide, D, groups, i):
+    """Values that are 1 in one feature (key j: feature j mod D groups, when that is among the i-th D), and what equal
+    weights make of them: the feature's visible keys over all visible keys."""
+    keys = hide.shape[1]
+    at = torch.arange(keys, device="cuda") % (D * groups) - i * D
+    v = torch.zeros(keys, D, device="cuda", dtype=torch.float64)
+    j = torch.nonzero((at >= 0) & (at < D))[:, 0]
+    v[j, at[j]] = 1.0
+    see = (~hide).double()
+    return v, see @ v / see.sum(1, keepdim=True)
+
+
+def counted(got, want):
+    """Equal scores make every weight exactly 1, so that sums are whole numbers: the division's rounding (2^-23) and the
+    output's. A feature has at most 32 keys: one of them too few or too many is off by a 33rd."""
+    return bool(((got.double() - want).abs() <= want * (2.0 ** -8 + 2.0 ** -22)).all())
+
+
+@pytest.mark.parametrize("hkv,rep,D", [(8, 4, 128), (2, 7, 64), (1, 1, 80), (2, 12, 128), (2, 2, 256), (1, 12, 192),
+                                       (1, 16, 16)])
+@pytest.mark.parametrize("n,pos", [(1, 0), (1, 14), (1, 15), (1, 16), (1, 127), (1, 128), (1, 2191), (1, 4100),
+                                   (1, 32767), (2, 1000), (3, 8190), (40, 2000), (150, 700), (700, 130)])
+def test_attend_counts_every_key(gen, n, pos, hkv, rep, D):
+    if n * rep * hkv * (pos + n) > 8e7:
+        n = max(1, int(8e7 / (rep * hkv * (pos + n))))
+    total = pos + n
+    c = cache(gen, hkv, D, total + 5, total)
+    q = torch.zeros(n, hkv * rep, D, device="cuda", dtype=torch.bfloat16)
+    hide = ~seen(torch.arange(pos, total, device="cuda")[:, None], torch.arange(total, device="cuda")[None], 0, 0)
+    groups = -(-total // (32 * D))
+    for i in range(groups):
+        v, want = counts(hide, D, groups, i)
+        put(c, v=v.to(torch.bfloat16).expand(hkv, -1, -1).contiguous())
+        out = c.attend(q, pos, cuda.attn_config(hkv * rep))
+        assert counted(out, want[:, None]), i
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n,pos,window,sinks,slack", [(1, 1000, 24, 4, 3), (1, 9000, 4096, 4, 0), (3, 700, 65, 1, 0),
+                                                      (64, 640, 128, 0, 0), (200, 1999, 300, 130, 5), (9, 0, 40, 4, 0),
+                                                      (257, 5000, 1024, 4, 77), (512, 3000, 700, 17, 0)])
+def test_attend_ring_counts_every_key(gen, n, pos, window, sinks, slack, D):
+    total = pos + n
+    c = cache(gen, 2, D, sinks + window + n - 1 + slack, total, window, sinks)
+    q = torch.zeros(n, 8, D, device="cuda", dtype=torch.bfloat16)
+    hide = ~seen(torch.arange(pos, total, device="cuda")[:, None], torch.arange(total, device="cuda")[None], window, sinks)
+    groups = -(-(window + sinks) // (31 * D))
+    for i in range(groups):
+        v, want = counts(hide, D, groups, i)
+        put(c, v=v.to(torch.bfloat16).expand(2, -1, -1).contiguous())
+        out = c.attend(q, pos, cuda.attn_config(8, window=window, sinks=sinks))
+        assert counted(out, want[:, None]), i
+
+
+@pytest.mark.parametrize("hkv,rep,D", [(2, 4, 128), (8, 4, 128), (1, 12, 64), (2, 3, 256)])
+@pytest.mark.parametrize("seqs,prefix,tail", [(1, 1, 5), (3, 0, 300), (8, 1025, 64), (37, 517, 130), (24, 3000, 1000)])
+def test_shared_prefix_counts_every_key(gen, hkv, rep, D, seqs, prefix, tail):
+    t = Group(gen, hkv, D, prefix, prefix + 19, seqs, tail, layers=1, layer=0)
+    lens = [int(x) for x in torch.randint(1, tail + 1, (seqs,), device="cuda", generator=gen)]
+    lens[-1] = tail
+    if seqs > 2:
+        lens[1], lens[2] = 0 if prefix else 1, 17
+    q = torch.zeros(seqs, hkv * rep, D, device="cuda", dtype=torch.bfloat16)
+    groups = -(-(prefix + tail) // (32 * D))
+    ld = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    hide = torch.arange(prefix + tail, device="cuda")[None] >= prefix + ld[:, None]
+    for i in range(groups):
+        v, want = counts(hide, D, groups, i)
+        vb = v.to(torch.bfloat16).expand(hkv, -1, -1)
+        if prefix:
+            t.kv.write(0, 0, t.k, vb[:, :prefix].contiguous())
+        t.tv = vb[None, :, prefix:].expand(seqs, -1, -1, -1)
+        t.fill(lens)
+        assert counted(t.attend(q, ld, cuda.attn_config(hkv * rep)), want[:, None]), i
+
+
+# ------------------------------------------------------------------ maxima that rise along the keys
+
+def rising(c, q, pos, scale, window=0, sinks=0):
+    """Keys whose size grows along the positions, so that the rows' maxima jump again and again, and values that shrink
+    by as much as the weights grow, so that what was summed before each jump counts in the result."""
+    total = c.k.shape[1]
+    g = 0.2 + 5.0 * torch.arange(total, device="cuda") / total
+    sigma = q.double().pow(2).sum(-1).mean().sqrt() * scale      # of a score over keys of size 1
+    k = (c.k.double() * g[:, None]).to(torch.bfloat16)
+    v = (c.v.double() * torch.exp(3.0 * sigma * (g[-1] - g))[:, None]).to(torch.bfloat16)
+    put(c, k, v)
+
+
+@pytest.mark.parametrize("hkv,rep,D,n,pos", [(2, 8, 128, 1777, 1223), (2, 8, 64, 1777, 1223), (2, 8, 80, 1500, 900),
+                                             (1, 32, 128, 300, 5000), (1, 32, 64, 300, 5000), (1, 16, 128, 40, 16000),
+                                             (1, 16, 64, 41, 9001), (5, 4, 128, 1990, 200), (2, 4, 128, 1, 5000),
+                                             (2, 4, 128, 2, 5000), (2, 4, 256, 40, 3000), (1, 12, 256, 1, 3000)])
+def test_attend_rising_maxima(gen, hkv, rep, D, n, pos):
+    c = cache(gen, hkv, D, pos + n + 3, pos + n)
+    q = rand(gen, n, hkv * rep, D, scale=1.5)
+    rising(c, q, pos, D ** -0.5)
+    c.check(c.attend(q, pos, cuda.attn_config(hkv * rep)), q, pos, heads=sorted({0, rep - 1, hkv * rep - 1}))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n,pos,window,sinks", [(512, 7680, 4096, 4), (1200, 6000, 1500, 4)])
+def test_attend_ring_rising_maxima(gen, n, pos, window, sinks, D):
+    c = cache(gen, 2, D, sinks + window + n - 1, pos + n, window, sinks)
+    q = rand(gen, n, 16, D, scale=1.5)
+    rising(c, q, pos, D ** -0.5)
+    c.check(c.attend(q, pos, cuda.attn_config(16, window=window, sinks=sinks)), q, pos, window, sinks, heads=[0, 7, 9])
+
+
+@pytest.mark.parametrize("n", [150, 1500])
+def test_attend_extreme_scores_in_value(gen, n):
+    """Scores of +-2000 over many tiles: what the 64-bit form gives, not finiteness alone."""
+    c = cache(gen, 2, 64, 400 + n, 300 + n)
+    q = rand(gen, n, 16, 64, scale=60.0)
+    c.check(c.attend(q, 300, cuda.attn_config(16)), q, 300, heads=[0, 5, 15])
+
+
+# ------------------------------------------------------------------ few rows: weights as two bf16 terms
+
+def pair_tolerance(q, k, v, hide, scale, out, parts):
+    """Weights off by 2 * 2^-17, scores as above, and f32 sums of at most keys / (16 parts) + 64 steps, each off by 2^-22
+    (a truncated product of 16 keys); then the output's rounding."""
+    z = q.double() @ k.double().T * scale
+    w = torch.softmax(z.masked_fill(hide, -math.inf), -1)
+    za = (q.double().abs() @ k.double().abs().T * scale).masked_fill(hide, 0).amax(-1, keepdim=True)
+    D, keys = k.shape[1], k.shape[0]
+    delta = (D + 4) * 2.0 ** -24 * za + 2.0 ** -20
+    return (w @ v.double().abs()) * (2.0 ** -16 + 2 * delta + (keys / (16 * parts) + 64) * 2.0 ** -22) + out.abs() * 2.0 ** -8
+
+
+@pytest.mark.parametrize("hkv,rep,D,n,pos", [(8, 4, 128, 1, 300), (8, 4, 128, 1, 2191), (8, 4, 128, 1, 32767),
+                                             (2, 8, 128, 1, 2191), (2, 8, 64, 1, 900), (1, 1, 80, 1, 500),
+                                             (2, 4, 128, 2, 1500), (1, 8, 256, 1, 1000), (1, 3, 192, 2, 700)])
+def test_attend_few_rows_keep_the_low_terms(gen, hkv, rep, D, n, pos):
+    c = cache(gen, hkv, D, pos + n, pos + n)
+    q = rand(gen, n, hkv * rep, D, scale=1.5)
+    out = c.attend(q, pos, cuda.attn_config(hkv * rep))
+    hide = ~seen(torch.arange(pos, pos + n, device="cuda")[:, None], torch.arange(pos + n, device="cuda")[None], 0, 0)
+    for h in range(hkv * rep):
+        k, v = c.k[h // rep], c.v[h // rep]
+        want, _ = attn_row(q[:, h], k, v, hide, D ** -0.5)
+        err = (out[:, h].double() - want).abs()
+        tol = pair_tolerance(q[:, h], k, v, hide, D ** -0.5, want, 8)
+        assert bool((err <= tol).all()), (h, float((err / tol).max()))
+
+
+def test_shared_prefix_tails_keep_the_low_terms(gen):
+    """No prefix: the tails' kernel alone."""
+    t = Group(gen, 2, 128, 0, 8, 6, 700, layers=1, layer=0)
+    lens = [1, 700, 33, 128, 499, 16]
+    t.fill(lens)
+    q = rand(gen, 6, 8, 128, scale=1.5)
+    out = t.attend(q, torch.tensor(lens, dtype=torch.int32, device="cuda"), cuda.attn_config(8))
+    for i, m in enumerate(lens):
+        for h in range(8):
+            k, v = t.tk[i, h // 4, :m], t.tv[i, h // 4, :m]
+            hide = torch.zeros(1, m, dtype=torch.bool, device="cuda")
+            want, _ = attn_row(q[i, h:h + 1], k, v, hide, 128 ** -0.5)
+            err = (out[i, h:h + 1].double() - want).abs()
+            assert bool((err <= pair_tolerance(q[i, h:h + 1], k, v, hide, 128 ** -0.5, want, 4)).all()), (i, h)
