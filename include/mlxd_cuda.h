@@ -236,7 +236,7 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    capacity - cache sinks - window + 1 queries a call, and no more sinks than
    the cache keeps. Scores, softmax statistics and sums are f32; the weights
    enter the value product rounded to bf16 (with at most 8 query rows per kv
-   head, a token's usual group, as two bf16 terms). A non-finite value row
+   head, a token's usual group, as two bf16 terms) and sum to one as they enter. A non-finite value row
    that one query sees may reach other queries of the same call; a NaN query
    stays alone. Every wait inside is bounded: a launch that gave up makes the
    next call on any cache fail once. */

@@ -628,9 +628,12 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 //                      V as stored: its rows are the contraction);
 //   warps 4-7, 8-11    query tile 0 / 1, one row per thread: maximum and sum
 //                      of S over the key tile, P = e^(S - m) rounded to bf16
-//                      over S's own columns. O is rescaled only when a row's
-//                      maximum grew by more than 2^8 (the statistics are
-//                      relative to the maximum in use, so any will do).
+//                      over S's own columns. The sum is of the rounded
+//                      weights: with a maximum in use below the true one the
+//                      largest is not 1, and a row's weights have to sum to
+//                      one as they enter the product. O is rescaled only when
+//                      a row's maximum grew by more than 2^8 (the statistics
+//                      are relative to the maximum in use, so any will do).
 //
 // While one query tile is in its softmax the tensor cores work on the other.
 // Per key tile and 256 rows the MMAs take 2048 clocks and the exponentials as
@@ -903,11 +906,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             };
             // weights of 32 keys relative to the maximum in use, and their sums
             uint32_t pk[32];
-            uint64_t add[2];
+            float add[4];
             auto weigh = [&](int w) {
                 const float mu = m == -INFINITY ? 0.f : m * s2;
                 const uint64_t ss = pair2(s2, s2), mm = pair2(-mu, -mu);
-                if (!(w & 1)) add[0] = add[1] = pair2(0.f, 0.f);
+                if (!(w & 1)) add[0] = add[1] = add[2] = add[3] = 0.f;
 #pragma unroll
                 for (int x = 16 * (w & 1); x < 16 * (w & 1) + 16; x++) {
                     const int y = 2 * (x % 16);
@@ -916,7 +919,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                     e0 = ex2(e0);
                     e1 = ex2(e1);
                     pk[x] = cvt_bf2(e0, e1);
-                    add[x & 1] = add2(add[x & 1], pair2(e0, e1));
+                    add_bf2(add[2 * (x & 1)], add[2 * (x & 1) + 1], pk[x]);
                 }
             };
 #pragma unroll
@@ -974,8 +977,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             for (int h = 0; h < 2; h++) {
                 if (h == 1) weigh(2);
                 weigh(2 * h + 1);
-                l[0] = add2(l[0], add[0]);
-                l[1] = add2(l[1], add[1]);
+                l[0] = add2(l[0], pair2(add[0], add[1]));
+                l[1] = add2(l[1], pair2(add[2], add[3]));
                 tmem_st32(ts + 32 * h, pk);
                 tmem_wait_st();
                 tc_fence_before();

@@ -1,5 +1,5 @@
-"""Attention over a cache and of a shared prefix where the plain comparison is blind: every key is counted once,
-maxima that rise along the keys, the bf16 pairs of few rows; against 64-bit forms.
+"""Attention over a cache and of a shared prefix where the plain comparison is blind: every key is counted once, the
+weights sum to one, maxima that rise along the keys, the bf16 pairs of few rows; against 64-bit forms.
 
 Tolerances: a rounding to bf16 is off by at most 2^-8 of the value. Weights rounded to bf16 over the sum of the same
 rounded weights move the normalised weights by at most 2 * 2^-8, weights held as two bf16 terms (8 + 8 bits and a sign)
@@ -160,6 +160,25 @@ def test_attend_extreme_scores_in_value(gen, n):
     c = cache(gen, 2, 64, 400 + n, 300 + n)
     q = rand(gen, n, 16, 64, scale=60.0)
     c.check(c.attend(q, 300, cuda.attn_config(16)), q, 300, heads=[0, 5, 15])
+
+
+# ------------------------------------------------------------------ weights that sum to one
+
+@pytest.mark.parametrize("hkv,rep,D,n,pos", [(2, 8, 128, 1777, 1223), (2, 8, 64, 700, 1223), (1, 32, 128, 300, 2000),
+                                             (1, 16, 128, 40, 9000), (2, 4, 128, 1, 3001), (2, 16, 256, 30, 1000)])
+def test_attend_of_equal_values_is_that_value(gen, hkv, rep, D, n, pos):
+    """Whatever the weights are: f32 sums of the weights as they enter the product leave less than half a step."""
+    c = cache(gen, hkv, D, pos + n, pos + n)
+    q = rand(gen, n, hkv * rep, D, scale=1.5)
+    total = pos + n
+    # a few keys stand out by 4 to 7 bits late in the row, where the maximum in use stays an earlier one
+    k = c.k.clone()
+    k[:, ::301] *= 2.0
+    one = rand(gen, hkv, 1, D).expand(-1, total, -1).contiguous()
+    put(c, k, one)
+    out = c.attend(q, pos, cuda.attn_config(hkv * rep))
+    want = one[:, 0].repeat_interleave(rep, 0)
+    assert torch.equal(out, want.expand(n, -1, -1))
 
 
 # ------------------------------------------------------------------ few rows: weights as two bf16 terms
