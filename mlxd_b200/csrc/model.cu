@@ -1013,9 +1013,9 @@ static int kv_rows(mlxd_kv *kv, int layer, bool value, int pos, int n, uint16_t 
         set_error("kv rows: bad arguments");
         return -1;
     }
-    const int ring = kv->cap - kv->sinks;
-    if (pos >= kv->sinks && n > ring) {
-        set_error("kv rows: %d rows over a ring of %d slots", n, ring);
+    const int ring = kv->cap - kv->sinks, in_ring = pos < kv->sinks ? n - (kv->sinks - pos) : n;
+    if (in_ring > ring) {                            // two of the rows would share a slot
+        set_error("kv rows: %d rows over a ring of %d slots", in_ring, ring);
         return -1;
     }
     const size_t layer_elems = (size_t)kv->hkv * kv->cap * kv->d, row = (size_t)kv->d * 2;

@@ -224,3 +224,30 @@ def test_shared_prefix_tails_keep_the_low_terms(gen):
             want, _ = attn_row(q[i, h:h + 1], k, v, hide, 128 ** -0.5)
             err = (out[i, h:h + 1].double() - want).abs()
             assert bool((err <= pair_tolerance(q[i, h:h + 1], k, v, hide, 128 ** -0.5, want, 4)).all()), (i, h)
+
+
+# ------------------------------------------------------------------ cache rows
+
+def rows_refused(rc, word):
+    msg = cuda.lib().mlxd_cuda_last_error().decode()
+    assert rc == -1 and word in msg, (rc, msg)
+
+
+def test_cache_rows_that_share_slots_are_refused(gen):
+    """Rows from inside the sinks that reach round the whole ring: later positions would lie where the first do."""
+    L, hkv, D, cap, sinks = cuda.lib(), 2, 64, 14, 4
+    kv = cuda.KVCache.shaped(1, hkv, D, cap, window=10, sinks=sinks)
+    x = rand(gen, hkv, cap, D)
+    out = torch.full_like(x, 7.0)
+    for pos, n in ((0, 14), (2, 12), (3, 11), (4, 10), (40, 10)):
+        y = x[:, :n].contiguous()
+        kv.write(0, pos, y, -y)
+        o = torch.empty_like(y)
+        cuda.check(L.mlxd_cuda_kv_gather(kv.kv, 0, 1, pos, n, o.data_ptr(), None), "gather")
+        torch.cuda.synchronize()
+        assert torch.equal(o, -y)
+    for pos, n in ((1, 14), (2, 13), (3, 14), (4, 11)):
+        rows_refused(L.mlxd_cuda_kv_write(kv.kv, 0, pos, n, x.data_ptr(), x.data_ptr(), None), "over a ring of 10 slots")
+        rows_refused(L.mlxd_cuda_kv_gather(kv.kv, 0, 0, pos, n, out.data_ptr(), None), "over a ring of 10 slots")
+    torch.cuda.synchronize()
+    assert bool((out == 7).all())
