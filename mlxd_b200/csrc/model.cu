@@ -1009,7 +1009,7 @@ int mlxd_cuda_kv_reset(mlxd_kv *kv) {
 // slot p below `sinks`, the other slots the ring of the positions above)
 static int kv_rows(mlxd_kv *kv, int layer, bool value, int pos, int n, uint16_t *dev, bool to_cache,
                    cudaStream_t st) {
-    if (!kv || layer < 0 || layer >= kv->layers || pos < 0 || n < 0 || n > kv->cap || !dev) {
+    if (!kv || layer < 0 || layer >= kv->layers || pos < 0 || n < 0 || n > kv->cap || n > INT32_MAX - pos || !dev) {
         set_error("kv rows: bad arguments");
         return -1;
     }

@@ -251,3 +251,12 @@ def test_cache_rows_that_share_slots_are_refused(gen):
         rows_refused(L.mlxd_cuda_kv_gather(kv.kv, 0, 0, pos, n, out.data_ptr(), None), "over a ring of 10 slots")
     torch.cuda.synchronize()
     assert bool((out == 7).all())
+
+
+def test_cache_rows_past_the_last_position_are_refused(gen):
+    L = cuda.lib()
+    x = rand(gen, 2, 8, 64)
+    for kv in (cuda.KVCache.shaped(1, 2, 64, 14, window=10, sinks=4), cuda.KVCache.shaped(1, 2, 64, 9)):
+        for pos, n in ((2 ** 31 - 1, 1), (2 ** 31 - 4, 8)):
+            rows_refused(L.mlxd_cuda_kv_write(kv.kv, 0, pos, n, x.data_ptr(), x.data_ptr(), None), "bad arguments")
+            rows_refused(L.mlxd_cuda_kv_gather(kv.kv, 0, 0, pos, n, x.data_ptr(), None), "bad arguments")
