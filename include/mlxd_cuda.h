@@ -227,7 +227,11 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    q_i . k_j) v_j over the keys j <= pos + i that lie in the window
    (pos + i - j < window; window 0: every key) or among the first `sinks`
    positions. The rows of every visible position must have been written;
-   other rows may hold anything. q: bf16 [n][n_heads][head_dim] with
+   other rows may hold anything. Refused are positions that no kv_write or
+   model call has reached in this layer, and visible ones whose rows a ring has
+   overwritten since (writes that a captured graph makes are known from its
+   capture, when it runs is not: they overwrite nothing for this check, and a
+   captured call is not refused for overwritten rows). q: bf16 [n][n_heads][head_dim] with
    q_stride elements between tokens, out likewise; both 16-byte aligned, the
    strides multiples of 8 elements and at least n_heads * head_dim; q, out, ws
    and the cache must not overlap. Query head h reads kv head h / (n_heads / n_kv_heads). ws: a device workspace of
@@ -253,7 +257,9 @@ int  mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_
 
 /* A batch of sequences that share a prefix (n samples of one prompt; no
    reference counterpart): positions [0, prefix_len) are rows of `prefix`
-   (unwrapped, unchanged and alive while the group is), each sequence's
+   (unchanged and alive while the group is; a ring that has overwritten some of
+   them is refused here and by the group's attend, which refuses positions
+   that were never written, too), each sequence's
    further positions are rows of its own tail of up to tail_capacity tokens,
    held by the group. */
 typedef struct mlxd_kv_group mlxd_kv_group;

@@ -20,6 +20,7 @@ void dev_free(void *p);
 // p is aligned memory of the current device (device or managed); false + error
 // naming `what` otherwise (host memory, another device's, null)
 bool on_device(const void *p, const char *what, int align = 1);
+bool is_capturing(cudaStream_t st);
 
 // A projection in device memory. Every quantized matrix keeps its MLX
 // arrays (w u32 [rows][cols/8], scales/biases [rows][cols/group] of sdtype);
@@ -138,6 +139,16 @@ struct mlxd_kv {
     int att_nbmax = 0, att_rep = 0;   // att_rep 0: a cache of kv_create_shape
     CUtensorMap map_k, map_v;   // all layers' rows for kv_attend's tiles
     bool maps = false;
+    // What the host has written, per layer: positions up to `ever`; of those above the sinks [lost, end) lie in
+    // the ring now. Copies in a captured graph count only for `ever` (when the graph will run is not known).
+    struct Held {
+        int ever, end, lost;
+    };
+    Held *held = nullptr;       // [layers]
+
+    void wrote(int layer, int pos, int n, bool captured);
+    // the rows of [low, total), low above the sinks: null, or what is missing
+    const char *missing(int layer, int low, int total, bool captured) const;
 };
 
 // n sequences over a shared prefix: tails [L][n][hkv][cap][d]

@@ -51,7 +51,7 @@ MLXD_DEV int query_pos(const AttnCall &c, int i) {
     const int len = min(c.lens[i], c.tcap);
     return len < 0 ? -1 : c.prefix + len - 1;
 }
-MLXD_DEV int window_lo(const AttnCall &c, int p) { return c.window ? max(0, p - c.window + 1) : 0; }
+__host__ MLXD_DEV int window_lo(const AttnCall &c, int p) { return c.window && p >= c.window ? p - c.window + 1 : 0; }
 
 // The slots that hold positions [lo, hi) and the sinks below lo: [0, a1),
 // [c0, c1) (the wrapped end of a ring) and [b0, b1), ascending. In a wrapped
@@ -1413,6 +1413,12 @@ int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_s
             return -1;
         }
     }
+    // of what the queries see, the lowest position that no sink slot keeps
+    const int lo = window_lo(c, pos), low = lo <= kv->sinks || c.sinks > kv->sinks ? kv->sinks : lo;
+    if (const char *why = kv->missing(layer, low, total, is_capturing((cudaStream_t)stream))) {
+        set_error("kv_attend: positions %d to %d of layer %d %s", low, total - 1, layer, why);
+        return -1;
+    }
     if (!same_device(kv->device, "kv_attend") || gave_up("kv_attend")) return -1;
     const size_t layer_elems = (size_t)kv->hkv * kv->cap * kv->d;
     c.k = kv->k + layer * layer_elems;
@@ -1434,6 +1440,12 @@ int mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int pr
         set_error("kv_group_create: bad arguments");
         return -1;
     }
+    if (prefix_len > prefix->sinks)
+        for (int l = 0; l < prefix->layers; l++)
+            if (prefix->held[l].lost > prefix->sinks) {
+                set_error("kv_group_create: the prefix of layer %d has been overwritten by later positions", l);
+                return -1;
+            }
     if (!same_device(prefix->device, "kv_group_create")) return -1;
     mlxd_kv_group *g = new (std::nothrow) mlxd_kv_group();
     if (!g) {
@@ -1514,6 +1526,10 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
                               size_t ws_bytes, void *stream) try {
     if (!g || layer < 0 || layer >= g->layers) {
         set_error("kv_group_attend: bad arguments");
+        return -1;
+    }
+    if (const char *why = g->prefix->missing(layer, g->prefix->sinks, g->prefix_len, is_capturing((cudaStream_t)stream))) {
+        set_error("kv_group_attend: positions of the prefix of %d in layer %d %s", g->prefix_len, layer, why);
         return -1;
     }
     AttnCall c = {};

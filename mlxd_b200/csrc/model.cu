@@ -587,6 +587,7 @@ static int forward_dev(mlxd_model *m, mlxd_kv *kv, const int32_t *ids_dev, int n
     else
         rc = generic_forward(m, kv, ids_dev, n, want_logits, logits_out, st);
     if (rc) return -1;
+    for (int l = 0; l < kv->layers; l++) kv->wrote(l, kv->offset, n, false);
     kv->offset += n;
     return 0;
 }
@@ -907,6 +908,12 @@ int mlxd_cuda_kv_create(mlxd_kv **out, const mlxd_model *m, int capacity) {
         delete kv;
         return -1;
     }
+    kv->held = new (std::nothrow) mlxd_kv::Held[kv->layers]();
+    if (!kv->held) {
+        set_error("kv_create: out of host memory");
+        delete kv;
+        return -1;
+    }
     size_t n = (size_t)kv->layers * kv->hkv * kv->cap * kv->d;
     kv->k = (uint16_t *)dev_alloc(n * 2);
     kv->v = (uint16_t *)dev_alloc(n * 2);
@@ -960,6 +967,12 @@ int mlxd_cuda_kv_create_shape(mlxd_kv **out, int layers, int n_kv_heads, int hea
     kv->window = window;
     kv->sinks = sinks;
     kv->offset = 0;
+    kv->held = new (std::nothrow) mlxd_kv::Held[layers]();
+    if (!kv->held) {
+        set_error("kv_create_shape: out of host memory");
+        delete kv;
+        return -1;
+    }
     const size_t bytes = (size_t)layers * n_kv_heads * capacity * head_dim * 2;
     if (!cuda_ok(cudaGetDevice(&kv->device), "kv_create_shape") || !(kv->k = (uint16_t *)dev_alloc(bytes)) ||
         !(kv->v = (uint16_t *)dev_alloc(bytes)) || !(kv->d_pos = (int32_t *)dev_alloc(4)) ||
@@ -983,6 +996,7 @@ void mlxd_cuda_kv_destroy(mlxd_kv *kv) {
     dev_free(kv->d_pos);
     dev_free(kv->att_part);
     dev_free(kv->att_cnt);
+    delete[] kv->held;
     delete kv;
 }
 
@@ -999,9 +1013,34 @@ int mlxd_cuda_kv_capacity(const mlxd_kv *kv, int layer) {
 int mlxd_cuda_kv_reset(mlxd_kv *kv) {
     if (!kv) return -1;
     kv->offset = 0;
+    for (int l = 0; l < kv->layers; l++) kv->held[l].end = kv->held[l].lost = 0;
     MLXD_CHECK(cudaMemset(kv->d_pos, 0, 4));
     MLXD_CHECK(cudaDeviceSynchronize());
     return 0;
+}
+
+void mlxd_kv::wrote(int layer, int pos, int n, bool captured) {
+    Held &h = held[layer];
+    const int ring = cap - sinks, e = pos + n, p = pos < sinks ? sinks : pos;
+    if (!captured && e > p) {                        // (the sinks' slots are their own)
+        if (p < h.lost) {
+            // a lost position comes back, over the slots of the positions one ring later
+            if (e < h.lost) h.end = e;               // apart from what is held
+            else if ((int64_t)p + ring < h.end) h.end = p + ring;
+            h.lost = p;
+            h.ever = h.end;
+        }
+        if (e > h.end) h.end = e;
+        if (h.end - ring > h.lost) h.lost = h.end - ring;
+    }
+    if (n > 0 && e > h.ever) h.ever = e;
+}
+
+const char *mlxd_kv::missing(int layer, int low, int total, bool captured) const {
+    const Held &h = held[layer];
+    if (total > h.ever) return "have not been written";
+    if (!captured && low < (total < h.lost ? total : h.lost)) return "have been overwritten by later ones";
+    return nullptr;
 }
 
 // rows [pos, pos + n) of every kv head of one layer, ring-aware, as 2-D
@@ -1040,7 +1079,9 @@ int mlxd_cuda_kv_write(mlxd_kv *kv, int layer, int pos, int n, const void *k_dev
                        void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
     if (kv_rows(kv, layer, false, pos, n, (uint16_t *)k_dev, true, st)) return -1;
-    return kv_rows(kv, layer, true, pos, n, (uint16_t *)v_dev, true, st);
+    if (kv_rows(kv, layer, true, pos, n, (uint16_t *)v_dev, true, st)) return -1;
+    kv->wrote(layer, pos, n, is_capturing(st));
+    return 0;
 }
 
 int mlxd_cuda_kv_gather(mlxd_kv *kv, int layer, int is_value, int pos, int n, void *dst_dev, void *stream) {
@@ -1484,6 +1525,7 @@ int mlxd_cuda_generate_ctl(mlxd_model *m, mlxd_kv *kv, const int32_t *prompt, in
                 return -1;
             append_token_kernel<<<1, 1, 0, st>>>(m->ctx, n + e, m->token);
         }
+        for (int l = 0; l < kv->layers; l++) kv->wrote(l, kv->offset, 1, false);
         kv->offset += 1;
         MLXD_CHECK(cudaMemcpyAsync(pin + n + (e & 1), m->token, 4, cudaMemcpyDeviceToHost, st));
         if (logprobs) MLXD_CHECK(cudaMemcpyAsync(pin_lp + (e & 1), m->lp, 4, cudaMemcpyDeviceToHost, st));

@@ -58,6 +58,13 @@ void dev_free(void *p) {
     cudaFree(p);
 }
 
+bool is_capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st, &s) == cudaSuccess) return s != cudaStreamCaptureStatusNone;
+    cudaGetLastError();
+    return true;                                     // (the legacy stream while another one is captured)
+}
+
 typedef CUresult (*PointerGetAttributesFn)(unsigned, CUpointer_attribute *, void **, CUdeviceptr);
 
 bool on_device(const void *p, const char *what, int align) {

@@ -260,3 +260,119 @@ def test_cache_rows_past_the_last_position_are_refused(gen):
         for pos, n in ((2 ** 31 - 1, 1), (2 ** 31 - 4, 8)):
             rows_refused(L.mlxd_cuda_kv_write(kv.kv, 0, pos, n, x.data_ptr(), x.data_ptr(), None), "bad arguments")
             rows_refused(L.mlxd_cuda_kv_gather(kv.kv, 0, 0, pos, n, x.data_ptr(), None), "bad arguments")
+
+
+# ------------------------------------------------------------------ positions that a cache holds
+
+def attend_rc(kv, layer, q, pos, window=0, sinks=0, stream=None):
+    hq, D = q.shape[1:]
+    out = torch.empty_like(q)
+    ws = torch.empty(cuda.attn_workspace_bytes(D), dtype=torch.uint8, device="cuda")
+    rc = cuda.lib().mlxd_cuda_kv_attend(kv.kv, layer, q.data_ptr(), q.stride(0), q.shape[0], pos,
+                                        C.byref(cuda.attn_config(hq, window=window, sinks=sinks)), out.data_ptr(),
+                                        out.stride(0), ws.data_ptr(), ws.numel(), stream)
+    return rc, out, ws
+
+
+def test_attend_refuses_rows_that_a_models_ring_has_overwritten(gen):
+    cfg = cuda.synth_config(hidden=256, layers=2, n_heads=4, n_kv_heads=2, head_dim=64, inter=256, vocab=256,
+                            family=cuda.MISTRAL, window=16, max_pos=128)
+    m = cuda.Model(cfg, cuda.synth_host_tensors(cfg, seed=1))
+    kv = m.new_kv(24)
+    q = rand(gen, 2, 4, 64)
+    rows_refused(attend_rc(kv, 0, q, 0)[0], "have not been written")
+    m.forward(kv, list(range(9)))
+    for t in range(3):
+        m.forward(kv, [t])
+    assert attend_rc(kv, 1, q, 10)[0] == 0 and attend_rc(kv, 0, q, 3)[0] == 0
+    rows_refused(attend_rc(kv, 1, q, 11)[0], "have not been written")
+    g, short = cuda.KVGroup(kv, 12, 2, 4), cuda.KVGroup(kv, 13, 2, 4)
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+    def group(g):
+        out = torch.empty_like(q)
+        ws = torch.empty(cuda.attn_workspace_bytes(64), dtype=torch.uint8, device="cuda")
+        return cuda.lib().mlxd_cuda_kv_group_attend(g.g, 1, q.data_ptr(), 256, lens.data_ptr(),
+                                                    C.byref(cuda.attn_config(4)), out.data_ptr(), 256, ws.data_ptr(),
+                                                    ws.numel(), None)
+
+    assert group(g) == 0
+    rows_refused(group(short), "have not been written")
+    for a in range(12, 40, 7):
+        m.forward(kv, list(range(7)))
+    assert kv.offset() == 40
+    rows_refused(attend_rc(kv, 1, q, 10)[0], "have been overwritten")
+    rows_refused(attend_rc(kv, 0, q, 10, window=16)[0], "have been overwritten")
+    rows_refused(attend_rc(kv, 0, q, 22, window=8)[0], "have been overwritten")        # positions 15 to 23, 16 is held
+    assert attend_rc(kv, 0, q, 22, window=7)[0] == 0
+    assert attend_rc(kv, 0, q, 38, window=16)[0] == 0
+    rows_refused(group(g), "have been overwritten")
+    h = C.c_void_p(7)
+    rows_refused(cuda.lib().mlxd_cuda_kv_group_create(C.byref(h), kv.kv, 12, 2, 4), "has been overwritten")
+    assert h.value == 7
+    kv.reset()
+    m.forward(kv, list(range(9)))
+    assert attend_rc(kv, 1, q, 7)[0] == 0
+
+
+@pytest.mark.parametrize("sinks", [0, 3])
+def test_attend_takes_what_a_ring_holds_and_no_more(gen, sinks):
+    """Runs appended, taken back and written again in any order without gaps: an accepted call's positions lie in their
+    slots, and the run last written can always be attended to."""
+    D, ring = 8, 13
+    cap = sinks + ring
+    kv = cuda.KVCache.shaped(1, 1, D, cap, window=5, sinks=sinks)
+    r = torch.Generator().manual_seed(3)
+    roll = lambda a, b: int(torch.randint(a, b + 1, (1,), generator=r))  # noqa: E731
+    slot = lambda p: p if p < sinks else sinks + (p - sinks) % ring  # noqa: E731
+    x, held, end, seen_end, both = rand(gen, 1, cap, D), {}, 0, 0, set()
+    for i in range(600):
+        kind = roll(0, 9)
+        pos = end if kind < 7 else roll(0, end) if kind < 9 else 0
+        n = roll(1, min(ring, 6))
+        kv.write(0, pos, x[:, :n].contiguous(), x[:, :n].contiguous())
+        held.update({slot(p): p for p in range(pos, pos + n)})
+        end, seen_end = pos + n, max(seen_end, pos + n)
+        rows = min(n, 5)
+        if (end - rows >= sinks) or not sinks:
+            assert attend_rc(kv, 0, rand(gen, 1, 1, D), end - 1, window=rows)[0] == 0
+        for _ in range(4):
+            total, window, keep = roll(1, seen_end), roll(1, 5), roll(0, sinks)
+            want = set(range(max(0, total - window), total)) | set(range(min(keep, total)))
+            rc = attend_rc(kv, 0, rand(gen, 1, 1, D), total - 1, window=window, sinks=keep)[0]
+            ok = all(held.get(slot(p)) == p for p in want)
+            both.add((rc == 0, ok))
+            assert ok or rc == -1, (i, total, window, keep)
+    assert (True, True) in both and (False, False) in both
+
+
+def test_captured_writes_overwrite_nothing_before_they_run(gen):
+    """A graph of the next positions' writes and attention, captured ahead: earlier positions stay open to eager calls."""
+    D, window = 64, 10
+    kv = cuda.KVCache.shaped(1, 2, D, 14, window=window)
+    x, y, q = rand(gen, 2, 14, D), rand(gen, 2, 4, D), rand(gen, 1, 4, D)
+    kv.write(0, 0, x, x)
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    first = attend_rc(kv, 0, q, 9, window=window)[1]
+    out = torch.empty_like(q)
+    ws = torch.empty(cuda.attn_workspace_bytes(D), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        st = torch.cuda.current_stream().cuda_stream
+        kv.write(0, 14, y, y, st)
+        cuda.check(cuda.lib().mlxd_cuda_kv_attend(kv.kv, 0, q.data_ptr(), 256, 1, 17,
+                                                  C.byref(cuda.attn_config(4, window=window)), out.data_ptr(), 256,
+                                                  ws.data_ptr(), ws.numel(), st), "attend")
+    rc, again, _ = attend_rc(kv, 0, q, 9, window=window)
+    torch.cuda.synchronize()
+    assert rc == 0 and torch.equal(first, again)
+    g.replay()
+    torch.cuda.synchronize()
+    flat = cuda.KVCache.shaped(1, 2, D, 18)
+    flat.write(0, 0, torch.cat((x, y), 1), torch.cat((x, y), 1))
+    rc, want, _ = attend_rc(flat, 0, q, 17, window=window)
+    torch.cuda.synchronize()
+    assert rc == 0
+    # the same keys in another order of slots: f32 sums of a few terms, each weight off by at most 2 * 2^-17
+    bound = 2.0 ** -15 * x.double().abs().max() + 2.0 ** -7 * want.double().abs()
+    assert bool(((out.double() - want.double()).abs() <= bound).all())
