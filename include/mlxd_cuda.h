@@ -242,8 +242,8 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    enter the value product rounded to bf16 (with at most 8 query rows per kv
    head, a token's usual group, as two bf16 terms) and sum to one as they enter. A non-finite value row
    that one query sees may reach other queries of the same call; a NaN query
-   stays alone. Every wait inside is bounded: a launch that gave up makes the
-   next call on any cache fail once. */
+   stays alone. Every wait inside is bounded: a launch that gave up (its rows
+   are wrong) sets the cache's word, see kv_gave_up. */
 typedef struct {
     int   n_heads;             /* query heads, a multiple of the cache's kv heads */
     int   window;              /* > 0: keys within the last `window` positions */
@@ -254,6 +254,12 @@ size_t mlxd_cuda_attn_workspace_bytes(int head_dim);
 int  mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_stride, int n, int pos,
                          const mlxd_attn *a, void *out, int64_t out_stride, void *ws, size_t ws_bytes,
                          void *stream);
+/* The host word that an attention launch over this cache sets to 1 when it
+   gave up on a wait (NULL: the cache has none and takes no launch that waits).
+   To be read once the launch is complete; the only report of a graph's
+   replays. The next kv_attend on the cache fails once when it is set and
+   clears it; a caller that has read it may clear it, too. */
+int32_t *mlxd_cuda_kv_gave_up(const mlxd_kv *kv);
 
 /* A batch of sequences that share a prefix (n samples of one prompt; no
    reference counterpart): positions [0, prefix_len) are rows of `prefix`
@@ -286,6 +292,7 @@ int  mlxd_cuda_kv_group_append(mlxd_kv_group *g, int layer, const void *k, int64
 int  mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, int64_t q_stride,
                                const int32_t *lens_dev, const mlxd_attn *a, void *out, int64_t out_stride,
                                void *ws, size_t ws_bytes, void *stream);
+int32_t *mlxd_cuda_kv_group_gave_up(const mlxd_kv_group *g);   /* as kv_gave_up, of the group's launches */
 
 /* ---- sampler (sampler.h:11-50) ------------------------------------------ */
 typedef struct {

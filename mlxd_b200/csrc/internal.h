@@ -21,6 +21,9 @@ void dev_free(void *p);
 // naming `what` otherwise (host memory, another device's, null)
 bool on_device(const void *p, const char *what, int align = 1);
 bool is_capturing(cudaStream_t st);
+// a zeroed word of pinned host memory that kernels can write (nullptr: none to be had), and its return
+int *host_word();
+void host_word_free(int *w);
 
 // A projection in device memory. Every quantized matrix keeps its MLX
 // arrays (w u32 [rows][cols/8], scales/biases [rows][cols/group] of sdtype);
@@ -139,6 +142,7 @@ struct mlxd_kv {
     int att_nbmax = 0, att_rep = 0;   // att_rep 0: a cache of kv_create_shape
     CUtensorMap map_k, map_v;   // all layers' rows for kv_attend's tiles
     bool maps = false;
+    int *gave_up = nullptr;     // host word that a launch over this cache sets when a wait ran out
     // What the host has written, per layer: positions up to `ever`; of those above the sinks [lost, end) lie in
     // the ring now. Copies in a captured graph count only for `ever` (when the graph will run is not known).
     struct Held {
@@ -157,4 +161,5 @@ struct mlxd_kv_group {
     int prefix_len, n, cap;
     int layers, hkv, d, device;
     uint16_t *k = nullptr, *v = nullptr;
+    int *gave_up = nullptr;     // as the cache's
 };

@@ -7,7 +7,6 @@
 // the keys with a running maximum m_i.
 #include <limits.h>
 #include <math.h>
-#include <mutex>
 #include <new>
 #include <type_traits>
 
@@ -649,7 +648,8 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 // keys at a time (402 us), three key or value stages.
 // Keys no row of the CTA sees may hold anything: their scores are masked and
 // their value rows zeroed in shared memory. Every wait is bounded; a launch
-// that gave up says so in a host word that the next call reports.
+// that gave up says so in its cache's (or group's) host word, which the next
+// call over it reports.
 constexpr int AT_THREADS = 384, AT_KT = 128, AT_ROWS = 256;
 
 template <int DB, bool BK>
@@ -1199,27 +1199,12 @@ __global__ void group_append_kernel(const uint16_t *__restrict__ k, int64_t ks, 
     }
 }
 
-// a word in host memory that a launch sets when it gave up on a wait; made
-// with the first cache (null before), read at every call
-static int *fail_word(bool make) {
-    static std::mutex mu;
-    static int *word = nullptr;
-    std::lock_guard<std::mutex> lock(mu);
-    if (!word && make) {
-        if (cudaHostAlloc((void **)&word, 64, cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
-            cudaGetLastError();
-            word = nullptr;
-        } else {
-            *word = 0;
-        }
-    }
-    return word;
-}
-static bool gave_up(const char *what) {
-    volatile int *w = fail_word(false);
+// reports once that a launch over this cache or group gave up on a wait
+static bool gave_up(int *word, const char *what) {
+    volatile int *w = word;
     if (!w || !*w) return false;
     *w = 0;
-    set_error("%s: an earlier attention launch gave up waiting on its pipeline", what);
+    set_error("%s: an earlier attention launch over these rows gave up waiting on its pipeline", what);
     return true;
 }
 
@@ -1238,12 +1223,13 @@ static bool row_map(CUtensorMap *m, const uint16_t *base, int heads, int cap, in
 
 void kv_attend_prepare(mlxd_kv *kv) {
     // (no tiles without the word that reports their failures)
-    kv->maps = fail_word(true) && kv->d % 8 == 0 && kv->d <= 128 && row_map(&kv->map_k, kv->k, kv->layers * kv->hkv, kv->cap, kv->d) &&
+    kv->gave_up = host_word();
+    kv->maps = kv->gave_up && kv->d % 8 == 0 && kv->d <= 128 && row_map(&kv->map_k, kv->k, kv->layers * kv->hkv, kv->cap, kv->d) &&
                row_map(&kv->map_v, kv->v, kv->layers * kv->hkv, kv->cap, kv->d);
 }
 
 static int attend_tiles(const AttnCall &c, const mlxd_kv *kv, int layer, TileShape shape, bool partial, void *ws,
-                        cudaStream_t st) {
+                        int *fail, cudaStream_t st) {
     if (!kv->maps) {
         set_error("attention: the cache has no tensor maps (no cuTensorMapEncodeTiled, or no pinned host memory)");
         return -1;
@@ -1256,7 +1242,7 @@ static int attend_tiles(const AttnCall &c, const mlxd_kv *kv, int layer, TileSha
         t.part_o = (float *)ws;
         t.part_ml = at_ws_ml(ws, c.D);
     }
-    t.fail = fail_word(false);
+    t.fail = fail;
     if (c.D <= 64)
         return shape.by_keys ? launch_tile<1, true>(c, t, kv->map_k, kv->map_v, st)
                              : launch_tile<1, false>(c, t, kv->map_k, kv->map_v, st);
@@ -1275,7 +1261,7 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
             return -1;
         }
         const TileShape shape = tile_shape(c, keys);
-        if (attend_tiles(c, kv, layer, shape, shape.splits > 1, ws, st)) return -1;
+        if (attend_tiles(c, kv, layer, shape, shape.splits > 1, ws, kv->gave_up, st)) return -1;
         if (shape.splits == 1) return 0;
         c.part_o = (const float *)ws;
         c.part_ml = at_ws_ml(ws, c.D);
@@ -1299,7 +1285,7 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
 
 // sequences in batches whose partial rows fit the workspace: the prefix (on
 // tiles unless the heads are too wide), then every sequence's tail, which joins the prefix's results
-static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cudaStream_t st) {
+static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, int *fail, cudaStream_t st) {
     const int64_t tail = (int64_t)c.hkv * c.tcap * c.D;
     int64_t most = AT_WS_ROWS / c.hq < 65535 ? AT_WS_ROWS / c.hq : 65535;
     if (most < 1) {
@@ -1319,7 +1305,7 @@ static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
             if (attend_few(b, FEW_PREFIX, c.prefix, ws, st)) return -1;
         } else if (c.prefix > 0) {
             const TileShape shape = tile_shape(b, c.prefix);
-            if (attend_tiles(b, kv, layer, shape, true, ws, st)) return -1;
+            if (attend_tiles(b, kv, layer, shape, true, ws, fail, st)) return -1;
             b.part_o = (const float *)ws;
             b.part_ml = at_ws_ml(ws, c.D);
             b.parts = shape.splits;
@@ -1419,7 +1405,7 @@ int mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_s
         set_error("kv_attend: positions %d to %d of layer %d %s", low, total - 1, layer, why);
         return -1;
     }
-    if (!same_device(kv->device, "kv_attend") || gave_up("kv_attend")) return -1;
+    if (!same_device(kv->device, "kv_attend") || gave_up(kv->gave_up, "kv_attend")) return -1;
     const size_t layer_elems = (size_t)kv->hkv * kv->cap * kv->d;
     c.k = kv->k + layer * layer_elems;
     c.v = kv->v + layer * layer_elems;
@@ -1465,6 +1451,11 @@ int mlxd_cuda_kv_group_create(mlxd_kv_group **out, const mlxd_kv *prefix, int pr
         mlxd_cuda_kv_group_destroy(g);
         return -1;
     }
+    if (!(g->gave_up = host_word())) {
+        set_error("kv_group_create: no pinned host memory");
+        mlxd_cuda_kv_group_destroy(g);
+        return -1;
+    }
     *out = g;
     return 0;
 } catch (...) {   // no exception leaves a C entry
@@ -1477,8 +1468,12 @@ void mlxd_cuda_kv_group_destroy(mlxd_kv_group *g) {
     cudaDeviceSynchronize();
     dev_free(g->k);
     dev_free(g->v);
+    host_word_free(g->gave_up);
     delete g;
 }
+
+int32_t *mlxd_cuda_kv_gave_up(const mlxd_kv *kv) { return kv ? kv->gave_up : nullptr; }
+int32_t *mlxd_cuda_kv_group_gave_up(const mlxd_kv_group *g) { return g ? g->gave_up : nullptr; }
 
 int mlxd_cuda_kv_group_write(mlxd_kv_group *g, int layer, int seq, int row, int n, const void *k_dev,
                              const void *v_dev, void *stream) {
@@ -1535,7 +1530,7 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     AttnCall c = {};
     if (attn_call(c, "kv_group_attend", g->hkv, g->d, q, q_stride, g->n, a, out, out_stride, ws, ws_bytes) ||
         !on_device(lens_dev, "kv_group_attend: lengths", 4) || !same_device(g->device, "kv_group_attend") ||
-        gave_up("kv_group_attend"))
+        gave_up(g->gave_up, "kv_group_attend"))
         return -1;
     const size_t layer_elems = (size_t)g->hkv * g->prefix->cap * g->d;
     const size_t o = (size_t)layer * g->n * g->hkv * g->cap * g->d;
@@ -1547,7 +1542,7 @@ int mlxd_cuda_kv_group_attend(const mlxd_kv_group *g, int layer, const void *q, 
     c.tv = g->v + o;
     c.tcap = g->cap;
     c.prefix = c.total = g->prefix_len;
-    return attend_group(c, g->prefix, layer, ws, (cudaStream_t)stream);
+    return attend_group(c, g->prefix, layer, ws, g->gave_up, (cudaStream_t)stream);
 } catch (...) {   // no exception leaves a C entry
     set_error("kv_group_attend: out of host memory");
     return -1;

@@ -996,6 +996,7 @@ void mlxd_cuda_kv_destroy(mlxd_kv *kv) {
     dev_free(kv->d_pos);
     dev_free(kv->att_part);
     dev_free(kv->att_cnt);
+    host_word_free(kv->gave_up);
     delete[] kv->held;
     delete kv;
 }

@@ -58,6 +58,34 @@ void dev_free(void *p) {
     cudaFree(p);
 }
 
+// words 64 bytes apart, allocated a page at a time; a free one holds the next free one's address
+static std::mutex g_word_mu;
+static void *g_words = nullptr;
+
+int *host_word() {
+    std::lock_guard<std::mutex> lk(g_word_mu);
+    if (!g_words) {
+        char *page = nullptr;
+        if (cudaHostAlloc((void **)&page, 4096, cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        for (int o = 0; o < 4096; o += 64) *(void **)(page + o) = o + 64 < 4096 ? page + o + 64 : nullptr;
+        g_words = page;
+    }
+    int *w = (int *)g_words;
+    g_words = *(void **)w;
+    *(void **)w = nullptr;
+    return w;
+}
+
+void host_word_free(int *w) {
+    if (!w) return;
+    std::lock_guard<std::mutex> lk(g_word_mu);
+    *(void **)w = g_words;
+    g_words = w;
+}
+
 bool is_capturing(cudaStream_t st) {
     cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(st, &s) == cudaSuccess) return s != cudaStreamCaptureStatusNone;

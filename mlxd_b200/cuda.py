@@ -161,6 +161,8 @@ _SIGS = {
     "mlxd_cuda_attn_workspace_bytes": (C.c_size_t, [C.c_int]),
     "mlxd_cuda_kv_attend": (C.c_int, [P, C.c_int, P, C.c_int64, C.c_int, C.c_int,
                                       C.POINTER(AttnConfig), P, C.c_int64, P, C.c_size_t, P]),
+    "mlxd_cuda_kv_gave_up": (C.POINTER(C.c_int32), [P]),
+    "mlxd_cuda_kv_group_gave_up": (C.POINTER(C.c_int32), [P]),
     "mlxd_cuda_kv_group_create": (C.c_int, [C.POINTER(P), P, C.c_int, C.c_int, C.c_int]),
     "mlxd_cuda_kv_group_destroy": (None, [P]),
     "mlxd_cuda_kv_group_write": (C.c_int, [P, C.c_int, C.c_int, C.c_int, C.c_int, P, P, P]),

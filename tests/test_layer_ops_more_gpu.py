@@ -376,3 +376,44 @@ def test_captured_writes_overwrite_nothing_before_they_run(gen):
     # the same keys in another order of slots: f32 sums of a few terms, each weight off by at most 2 * 2^-17
     bound = 2.0 ** -15 * x.double().abs().max() + 2.0 ** -7 * want.double().abs()
     assert bool(((out.double() - want.double()).abs() <= bound).all())
+
+
+# ------------------------------------------------------------------ launches that gave up
+
+def test_a_launch_that_gave_up_is_reported_to_its_own_caller(gen):
+    """The words are set here as a launch would set them: no input makes a wait run out."""
+    L = cuda.lib()
+    a, b = (cache(gen, 2, 64, 300, 300) for _ in range(2))
+    ga, gb = (Group(gen, 2, 64, 100, 100, 2, 8, layers=1, layer=0) for _ in range(2))
+    q, lens, cfg = rand(gen, 40, 4, 64), torch.ones(2, dtype=torch.int32, device="cuda"), cuda.attn_config(4)
+    for t in (ga, gb):
+        t.fill([1, 1])
+    calls = [lambda: a.attend(q, 200, cfg), lambda: b.attend(q, 200, cfg), lambda: ga.attend(q[:2], lens, cfg),
+             lambda: gb.attend(q[:2], lens, cfg)]
+    words = [L.mlxd_cuda_kv_gave_up(a.kv.kv), L.mlxd_cuda_kv_gave_up(b.kv.kv), L.mlxd_cuda_kv_group_gave_up(ga.g.g),
+             L.mlxd_cuda_kv_group_gave_up(gb.g.g)]
+    assert len({C.addressof(w.contents) for w in words}) == 4
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    for i, w in enumerate(words):
+        assert [x[0] for x in words] == [0] * 4
+        w[0] = 1
+        for j, f in enumerate(calls):
+            if j == i:
+                with pytest.raises(cuda.CudaError, match="gave up"):
+                    f()
+            assert torch.equal(f(), want[j])
+    assert not L.mlxd_cuda_kv_gave_up(None) and not L.mlxd_cuda_kv_group_gave_up(None)
+
+
+def test_gave_up_words_come_and_go_with_their_caches(gen):
+    """More caches than one page of words serves, some destroyed with their word set: new ones begin with zero."""
+    L = cuda.lib()
+    for _ in range(3):
+        kvs = [cuda.KVCache.shaped(1, 1, 8, 4) for _ in range(150)]
+        words = [L.mlxd_cuda_kv_gave_up(kv.kv) for kv in kvs]
+        assert len({C.addressof(w.contents) for w in words}) == 150 and all(w[0] == 0 for w in words)
+        for w in words[::2]:
+            w[0] = 1
+        for kv in kvs:
+            kv.close()
