@@ -318,8 +318,8 @@ int mlxd_cuda_sample(const void *logits_dev, int dtype, int V, const mlxd_sampli
 /* Scores of given tokens (the raw logprob of sampler_sample_lazy,
    sampler.c:269-380, for any token of any row, with the distribution's
    entropy and its most likely tokens): for each of `rows` rows of V logits
-   (bf16 or f32, row_stride elements apart) logprobs[r] = log softmax(row)
-   [targets[r]], entropy[r] in nats, and the n_top (0 .. 32, at most V)
+   (below 2^31 - 256; bf16 or f32, row_stride elements apart) logprobs[r] =
+   log softmax(row)[targets[r]], entropy[r] in nats, and the n_top (0 .. 32, at most V)
    largest logits' ids in descending order, ties to the lower id, with their
    logprobs ([rows][n_top]). Statistics are f32 with the largest term kept
    apart, so that peaked rows lose nothing. Any output may be NULL; targets

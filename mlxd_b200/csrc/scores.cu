@@ -25,6 +25,7 @@
 namespace mlxd {
 
 constexpr int SC_THREADS = 256, SC_GROUPS = SC_THREADS / 4, SC_TOP = 32, SC_CAND = 1024, SC_MAXCL = 16;
+constexpr int SC_MAXV = INT32_MAX - SC_THREADS;      // a step of the CTA past the end is still an int
 // the first part: a quarter (a third 50.5, a sixth 53, an eighth 58 us: a looser T lists more)
 constexpr int SC_UNROLL = 4, SC_PART = 4;
 
@@ -573,9 +574,9 @@ using namespace mlxd;
 extern "C" int mlxd_cuda_token_scores(const void *logits, int dtype, int rows, int V, int64_t row_stride,
                                       const int32_t *targets, int n_top, float *logprobs, float *entropy,
                                       int32_t *top_ids, float *top_logprobs, void *stream) try {
-    if ((dtype != MLXD_BF16 && dtype != MLXD_F32) || rows < 0 || V <= 0 || row_stride < 0 || n_top < 0 ||
-        n_top > SC_TOP || n_top > V) {
-        set_error("token_scores: bad arguments (n_top: at most 32 and V)");
+    if ((dtype != MLXD_BF16 && dtype != MLXD_F32) || rows < 0 || V <= 0 || V > SC_MAXV || row_stride < 0 ||
+        n_top < 0 || n_top > SC_TOP || n_top > V) {
+        set_error("token_scores: bad arguments (n_top: at most 32 and V; V: below 2^31 - 256)");
         return -1;
     }
     if (logprobs && !targets) {

@@ -131,3 +131,8 @@ def test_cache_rows_refuse_strides_and_types():
     for b in (a.transpose(0, 1).contiguous().transpose(0, 1), a[:, ::2], a.float()):
         with pytest.raises(ValueError, match="cache rows"):
             cuda.row_count(b, b, (2, 16))
+
+
+@pytest.mark.parametrize("V", [2 ** 31 - 1, 2 ** 31 - 256])
+def test_scores_refuse_rows_whose_steps_pass_the_int_range(V):
+    refused(scores(V=V, stride=V), "token_scores: bad arguments")
