@@ -248,7 +248,7 @@ typedef struct {
     int   n_heads;             /* query heads, a multiple of the cache's kv heads */
     int   window;              /* > 0: keys within the last `window` positions */
     int   sinks;               /* with a window: first positions that stay visible */
-    float scale;               /* 0: 1 / sqrt(head_dim) */
+    float scale;               /* 1e-30 .. 1e30; 0: 1 / sqrt(head_dim) */
 } mlxd_attn;
 size_t mlxd_cuda_attn_workspace_bytes(int head_dim);
 int  mlxd_cuda_kv_attend(const mlxd_kv *kv, int layer, const void *q, int64_t q_stride, int n, int pos,

@@ -1319,8 +1319,8 @@ static int attend_group(AttnCall c, const mlxd_kv *kv, int layer, void *ws, int 
 static int attn_call(AttnCall &c, const char *what, int hkv, int D, const void *q, int64_t q_stride, int n,
                      const mlxd_attn *a, void *out, int64_t out_stride, const void *ws, size_t ws_bytes) {
     if (!a || a->n_heads <= 0 || a->n_heads % hkv || a->window < 0 || a->sinks < 0 || !(a->scale >= 0.f) ||
-        !isfinite(a->scale) || (a->scale > 0.f && a->scale < 1e-30f)) {
-        set_error("%s: bad attention parameters (heads a multiple of %d, window and sinks not negative, scale finite)",
+        a->scale > 1e30f || (a->scale > 0.f && a->scale < 1e-30f)) {
+        set_error("%s: bad attention parameters (heads a multiple of %d, window and sinks not negative, scale 0 or 1e-30 .. 1e30)",
                   what, hkv);
         return -1;
     }

@@ -417,3 +417,16 @@ def test_gave_up_words_come_and_go_with_their_caches(gen):
             w[0] = 1
         for kv in kvs:
             kv.close()
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_scale_range(gen, n):
+    """Scales whose product with log2 e leaves f32 are refused; the ends of the range weigh equal scores equally."""
+    c = cache(gen, 2, 64, 200, 200)
+    q = torch.zeros(n, 8, 64, device="cuda", dtype=torch.bfloat16)
+    want = c.attend(q, 100, cuda.attn_config(8))
+    for scale in (1e-30, 1.0, 1e30):
+        assert torch.equal(c.attend(q, 100, cuda.attn_config(8, scale=scale)), want)
+    for scale in (1e-31, 1e-45, 1.1e30, 3e38, math.inf, -1.0, math.nan):
+        with pytest.raises(cuda.CudaError, match="bad attention parameters"):
+            c.attend(q, 100, cuda.attn_config(8, scale=scale))
