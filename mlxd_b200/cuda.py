@@ -459,11 +459,12 @@ class Model:
 
 
 def row_count(k, v, shape):
-    """n of device arrays k and v, which must be contiguous [Hkv][n][D] of 2-byte elements (the
-    library sees their addresses alone)."""
+    """n of device arrays k and v, which must be contiguous [Hkv][n][D] of bf16 or of its bits as 16-bit
+    integers (the library sees their addresses alone)."""
     hkv, D = shape
     for a in (k, v):
-        if (tuple(a.shape) != (hkv, k.shape[1], D) or not a.is_contiguous() or a.element_size() != 2):
+        if (tuple(a.shape) != (hkv, k.shape[1], D) or not a.is_contiguous() or
+                str(a.dtype) not in ("torch.bfloat16", "torch.int16", "torch.uint16")):
             raise ValueError("cache rows: contiguous bf16 arrays [%d][n][%d], the same n for k and v" % (hkv, D))
     return k.shape[1]
 

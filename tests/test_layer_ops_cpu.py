@@ -136,3 +136,12 @@ def test_cache_rows_refuse_strides_and_types():
 @pytest.mark.parametrize("V", [2 ** 31 - 1, 2 ** 31 - 256])
 def test_scores_refuse_rows_whose_steps_pass_the_int_range(V):
     refused(scores(V=V, stride=V), "token_scores: bad arguments")
+
+
+def test_cache_rows_refuse_other_16_bit_floats():
+    a = torch.zeros(2, 5, 16, dtype=torch.bfloat16)
+    for b in (a, a.view(torch.int16), a.view(torch.uint16)):
+        assert cuda.row_count(b, b, (2, 16)) == 5
+    for k, v in ((a.half(), a), (a, a.half())):
+        with pytest.raises(ValueError, match="cache rows"):
+            cuda.row_count(k, v, (2, 16))
