@@ -212,8 +212,10 @@ def ptr(a):
 
 
 def dev_ptr(a):
-    """Device address of a DeviceBuffer or of a tensor with data_ptr()."""
-    return a.ptr if isinstance(a, DeviceBuffer) else C.c_void_p(a.data_ptr())
+    """Address of a tensor in device memory."""
+    if not a.is_cuda:
+        raise ValueError("a tensor in device memory is needed, not one on %s" % a.device)
+    return C.c_void_p(a.data_ptr())
 
 
 # ------------------------------------------------------------ device memory

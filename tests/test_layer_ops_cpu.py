@@ -145,3 +145,15 @@ def test_cache_rows_refuse_other_16_bit_floats():
     for k, v in ((a.half(), a), (a, a.half())):
         with pytest.raises(ValueError, match="cache rows"):
             cuda.row_count(k, v, (2, 16))
+
+
+def test_cache_rows_refuse_host_memory():
+    """Before the library is called with the address."""
+    kv = cuda.KVCache.__new__(cuda.KVCache)
+    kv.model, kv.kv, kv.shape = None, None, (2, 16)
+    g = cuda.KVGroup.__new__(cuda.KVGroup)
+    g.g, g.prefix = None, kv
+    a = torch.zeros(2, 5, 16, dtype=torch.bfloat16)
+    for f in (lambda: kv.write(0, 0, a, a), lambda: g.write(0, 0, 0, a, a)):
+        with pytest.raises(ValueError, match="device memory"):
+            f()
