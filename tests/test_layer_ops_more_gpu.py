@@ -7,10 +7,12 @@ by at most 2 * 2^-17. A score of D products in f32 is off by (D + 4) 2^-24 of su
 import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from mlxd_b200 import cuda
+from tests.helpers import bf16_to_f32
 from tests.test_layer_ops_gpu import Cache, Group, attn_row, rand, seen
 
 pytestmark = pytest.mark.gpu
@@ -430,3 +432,34 @@ def test_attend_scale_range(gen, n):
     for scale in (1e-31, 1e-45, 1.1e30, 3e38, math.inf, -1.0, math.nan):
         with pytest.raises(cuda.CudaError, match="bad attention parameters"):
             c.attend(q, 100, cuda.attn_config(8, scale=scale))
+
+
+# ------------------------------------------------------------------ rotary positions against the model's own
+
+@pytest.mark.parametrize("llama3", [None, (8.0, 1.0, 4.0, 64), (32.0, 1.0, 4.0, 8192)])
+def test_rope_turns_as_the_models_cache_rows(llama3):
+    """The same token at every position: the first layer's cached key at position 0 is the projection itself (cosine 1,
+    sine 0), the others are its rotations by the model's table. That one's angles are products in f32 (off by 2^-23 of
+    themselves), its cosines f32, the rows bf16; the op's angles are exact."""
+    n, D, hkv, theta = 300, 64, 2, 1e4
+    cfg = cuda.synth_config(hidden=256, layers=1, n_heads=4, n_kv_heads=hkv, head_dim=D, inter=256, vocab=256,
+                            family=cuda.LLAMA, theta=theta, llama3=llama3, max_pos=512)
+    m = cuda.Model(cfg, cuda.synth_host_tensors(cfg, seed=4, std=0.1))
+    kv = m.new_kv(n)
+    m.forward(kv, [7] * 200)
+    for _ in range(200, n):                      # the decode step's rows, too
+        m.forward(kv, [7])
+    rows = kv.read(0)                            # [hkv][n][D]
+    r = cuda.rope_config(theta, D)
+    if llama3:
+        r = cuda.rope_config(theta, D, scaling=cuda.ROPE_LLAMA3, factor=llama3[0], lo=llama3[1], hi=llama3[2],
+                             orig_max=llama3[3])
+    x = np.repeat(rows[None, :, 0], n, 0)        # [n][hkv][D]
+    got = bf16_to_f32(cuda.rope(x, r, 0)).astype(np.float64)
+    want = bf16_to_f32(rows).astype(np.float64).transpose(1, 0, 2)
+    a = np.abs(bf16_to_f32(x).astype(np.float64))
+    pair = np.concatenate((a[..., :D // 2] + a[..., D // 2:],) * 2, -1)
+    p = np.arange(n)[:, None, None]
+    bound = pair * (p * 2.0 ** -22 + 2.0 ** -20) + (np.abs(got) + np.abs(want)) * 2.0 ** -8
+    assert np.all(np.abs(got - want) <= bound)
+    assert np.abs(want).max() > 0.01 and not np.array_equal(want[1:], want[:-1])
