@@ -241,8 +241,8 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    the cache keeps. Scores, softmax statistics and sums are f32; the weights
    enter the value product rounded to bf16 (with at most 8 query rows per kv
    head, a token's usual group, as two bf16 terms) and sum to one as they enter. A non-finite value row
-   that one query sees may reach other queries of the same call; a NaN query
-   stays alone. Every wait inside is bounded: a launch that gave up (its rows
+   that one query sees may reach other queries of the same call (as NaN, where
+   it was infinite, too); a NaN query stays alone. Every wait inside is bounded: a launch that gave up (its rows
    are wrong) sets the cache's word, see kv_gave_up. */
 typedef struct {
     int   n_heads;             /* query heads, a multiple of the cache's kv heads */

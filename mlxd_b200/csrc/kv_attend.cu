@@ -81,8 +81,8 @@ MLXD_DEV int slot_pos(const AttnCall &c, int s) {
     return last - (d >= 0 ? d : d + ring);
 }
 
-// the partial results' room in a workspace: 148 CTAs of 256 rows, whatever
-// the call (more rows than that go unsplit, or in batches)
+// the partial results' room in a workspace: 148 CTAs (a B200's SMs) of 256 rows,
+// whatever the call (more rows than that go unsplit, or in batches)
 constexpr int64_t AT_WS_ROWS = 148 * 256;
 static size_t at_ws_bytes(int D) { return (size_t)AT_WS_ROWS * ((D + 7) / 8 * 8 * 4 + 8) + 256; }
 
@@ -589,7 +589,8 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
     if (s > FR_PARTS) s = FR_PARTS;
     if (s > AT_WS_ROWS / qrows) s = AT_WS_ROWS / qrows;
     if (s < 1) s = 1;
-    // more than two clusters' worth: partial results and a second kernel
+    // more than two clusters' worth: partial results and a second kernel; up to that one cluster, of a power of two
+    // (8 kv heads of 32: 4095 positions on 64 CTAs 11.7 us, 8191 on 144 14.9)
     const bool partial = kind == FEW_PREFIX || (kind == FEW_CACHE && s > 2 * FR_MAXCL);
     if (partial) {
         t.prow = qrows;
@@ -637,10 +638,11 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 // While one query tile is in its softmax the tensor cores work on the other.
 // Per key tile and 256 rows the MMAs take 2048 clocks and the exponentials as
 // many; the chain S -> maximum -> weights -> P V -> S of a query tile leaves some
-// 3700 (tensor pipe and exponentials 56% busy). A 4096-token chunk at 4096 of
-// 32/8 heads takes 379 us, 1087 TFLOP/s, 65% of the cuBLAS burst rate, at the
-// power limit (1.7 GHz); with the softmax left out the same MMAs took 328 us. The
-// first weights are taken by the old maximum while the new one is found, and
+// 3700 (tensor pipe and exponentials 57% busy). A 4096-token chunk at 4096 of
+// 32/8 heads takes 374 us, 1102 TFLOP/s, 65% of the cuBLAS burst rate, in runs of
+// a few ms, and 430 us (960 TFLOP/s) in seconds of them, at the power limit (985 W,
+// 1.7 GHz); with the softmax left out the same MMAs took 328 us. The softmax warps
+// spill 20 to 70 bytes a thread. The first weights are taken by the old maximum while the new one is found, and
 // again when it grew (398 -> 384 us). Tried without gain: exponentials of every
 // 3rd or 4th pair as a cubic on the FMA pipe, a row shared by two threads (500
 // us: four softmax warps to a scheduler wait for each other's maxima), the MMAs
@@ -1167,7 +1169,8 @@ static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &
 // over a 4096 window 60 us, against 69 in 256 rows and two splits, when this
 // was chosen; 51 now), beyond it
 // the latter, with half the loads per product (a 4096-token chunk 415 us, against
-// 514). Key splits fill the SMs when even those are few, no more than the key
+// 514). The step between them is steep: over a 4096 window 576 tokens of 32/8
+// heads (144 CTAs of 128 rows) take 50 us, 640 (80 of 256) 84, as 1024 do. Key splits fill the SMs when even those are few, no more than the key
 // tiles or the workspace's rows.
 struct TileShape {
     int by_keys, splits;
@@ -1268,7 +1271,9 @@ static int attend_cache(AttnCall c, const mlxd_kv *kv, int layer, void *ws, cuda
         c.parts = shape.splits;
         return launch_join(c, st);
     }
-    // few rows, or heads too wide for the tiles' accumulators: tokens in launches of at most 65535 items
+    // few rows, or heads wider than 128, for which the tiles have no form (two query tiles' accumulators would fill
+    // the TMEM; 4096 tokens at 4096 of 16/2 heads of 256 take 7.96 ms here, 52 TFLOP/s): tokens in launches of at most
+    // 65535 items
     int64_t most = (int64_t)(65535 / c.hkv) * 16 / c.rep;
     most = most < 1 ? 1 : most > 65535 ? 65535 : most;
     const int n = c.n;

@@ -12,7 +12,9 @@
 // tokens in shared memory, once per (token, pair) for all heads, then streams
 // the heads. 8192 tokens x 72 heads of 128 in bf16: 54 us, 85% of the measured
 // copy rate; 8 CTAs of 256 threads to an SM hide the loads' latency (4: 67 us,
-// 6: 60). A launch of one token is latency alone (2.6 us).
+// 6: 60). Rows that do not come in whole vectors go an element at a time: the
+// same prompt at an odd stride 165 us, 8192 x 32 heads of 80 with 40 turned 63 us
+// (floor 12.8). A launch of one token is latency alone (2.6 us).
 #include <math.h>
 
 #include "common.cuh"

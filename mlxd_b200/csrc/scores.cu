@@ -19,6 +19,7 @@
 // made from the whole row's group maxima. Measured, 512 rows of 151936 bf16 with
 // 20 alternatives: 50 us, 48% of the measured copy rate; 37 of them without the
 // sums, the rest of the distance the selection's serial steps at a row's end.
+// The same rows in f32: 67 us, 71%; 128 of them 49 us, 24% (fewer CTAs than SMs).
 #include "common.cuh"
 #include "kernels.h"
 
