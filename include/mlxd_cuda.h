@@ -322,7 +322,8 @@ int mlxd_cuda_sample(const void *logits_dev, int dtype, int V, const mlxd_sampli
    log softmax(row)[targets[r]], entropy[r] in nats, and the n_top (0 .. 32, at most V)
    largest logits' ids in descending order, ties to the lower id, with their
    logprobs ([rows][n_top]). Statistics are f32 with the largest term kept
-   apart, so that peaked rows lose nothing. Any output may be NULL; targets
+   apart, so that a peaked row's small logprob and entropy keep 18 bits of
+   their own. Any output may be NULL; targets
    may be NULL when logprobs is. -inf logits have probability zero; a row
    without any other is an empty distribution: logprobs -inf, entropy 0, top
    ids in index order. A row with +inf or NaN gives NaN scores (its ids order
