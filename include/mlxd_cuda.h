@@ -231,8 +231,8 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    model call has reached in this layer, and visible ones whose rows a ring has
    overwritten since (writes that a captured graph makes are known from its
    capture, when it runs is not: they overwrite nothing for this check, and a
-   captured call is not refused for overwritten rows). q: bf16 [n][n_heads][head_dim] with
-   q_stride elements between tokens, out likewise; both 16-byte aligned, the
+   captured call is not refused for overwritten rows). q: bf16
+   [n][n_heads][head_dim] with q_stride elements between tokens, out likewise; both 16-byte aligned, the
    strides multiples of 8 elements and at least n_heads * head_dim; q, out, ws
    and the cache must not overlap. Query head h reads kv head h / (n_heads / n_kv_heads). ws: a device workspace of
    attn_workspace_bytes(), 256-byte aligned, that no other call in flight
@@ -240,10 +240,11 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    capacity - cache sinks - window + 1 queries a call, and no more sinks than
    the cache keeps. Scores, softmax statistics and sums are f32; the weights
    enter the value product rounded to bf16 (with at most 8 query rows per kv
-   head, a token's usual group, as two bf16 terms) and sum to one as they enter. A non-finite value row
-   that one query sees may reach other queries of the same call (as NaN, where
-   it was infinite, too); a NaN query stays alone. Every wait inside is bounded: a launch that gave up (its rows
-   are wrong) sets the cache's word, see kv_gave_up. */
+   head, a token's usual group, as two bf16 terms) and sum to one as they
+   enter. A non-finite value row that one query sees may reach other queries of
+   the same call (as NaN, where it was infinite, too); a NaN query stays alone.
+   Every wait inside is bounded: a launch that gave up (its rows are wrong)
+   sets the cache's word, see kv_gave_up. */
 typedef struct {
     int   n_heads;             /* query heads, a multiple of the cache's kv heads */
     int   window;              /* > 0: keys within the last `window` positions */

@@ -642,8 +642,8 @@ static int attend_few(AttnCall &c, FewKind kind, int keys, void *ws, cudaStream_
 // 32/8 heads takes 374 us, 1102 TFLOP/s, 65% of the cuBLAS burst rate, in runs of
 // a few ms, and 430 us (960 TFLOP/s) in seconds of them, at the power limit (985 W,
 // 1.7 GHz); with the softmax left out the same MMAs took 328 us. The softmax warps
-// spill 20 to 70 bytes a thread. The first weights are taken by the old maximum while the new one is found, and
-// again when it grew (398 -> 384 us). Tried without gain: exponentials of every
+// spill 20 to 70 bytes a thread. The first weights are taken by the old maximum
+// while the new one is found, and again when it grew (398 -> 384 us). Tried without gain: exponentials of every
 // 3rd or 4th pair as a cubic on the FMA pipe, a row shared by two threads (500
 // us: four softmax warps to a scheduler wait for each other's maxima), the MMAs
 // of whichever tile is ready (704 us: both fall into phase), weights stored 32
@@ -1170,8 +1170,9 @@ static int launch_tile(const AttnCall &c, const TileCall &t, const CUtensorMap &
 // was chosen; 51 now), beyond it
 // the latter, with half the loads per product (a 4096-token chunk 415 us, against
 // 514). The step between them is steep: over a 4096 window 576 tokens of 32/8
-// heads (144 CTAs of 128 rows) take 50 us, 640 (80 of 256) 84, as 1024 do. Key splits fill the SMs when even those are few, no more than the key
-// tiles or the workspace's rows.
+// heads (144 CTAs of 128 rows) take 50 us, 640 (80 of 256) 84, as 1024 do. Key
+// splits fill the SMs when even those are few, no more than the key tiles or the
+// workspace's rows.
 struct TileShape {
     int by_keys, splits;
 };

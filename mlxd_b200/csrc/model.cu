@@ -1014,6 +1014,7 @@ int mlxd_cuda_kv_capacity(const mlxd_kv *kv, int layer) {
 int mlxd_cuda_kv_reset(mlxd_kv *kv) {
     if (!kv) return -1;
     kv->offset = 0;
+    // (`ever` stays: a graph captured before may write again)
     for (int l = 0; l < kv->layers; l++) kv->held[l].end = kv->held[l].lost = 0;
     MLXD_CHECK(cudaMemset(kv->d_pos, 0, 4));
     MLXD_CHECK(cudaDeviceSynchronize());
