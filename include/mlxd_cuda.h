@@ -232,11 +232,12 @@ int  mlxd_cuda_rope(const void *x, int dtype, int n, int heads, int head_dim, in
    overwritten since (writes that a captured graph makes are known from its
    capture, when it runs is not: they overwrite nothing for this check, and a
    captured call is not refused for overwritten rows). q: bf16
-   [n][n_heads][head_dim] with q_stride elements between tokens, out likewise; both 16-byte aligned, the
-   strides multiples of 8 elements and at least n_heads * head_dim; q, out, ws
-   and the cache must not overlap. Query head h reads kv head h / (n_heads / n_kv_heads). ws: a device workspace of
-   attn_workspace_bytes(), 256-byte aligned, that no other call in flight
-   uses (calls on one stream may share it). A wrapped ring takes at most
+   [n][n_heads][head_dim] with q_stride elements between tokens, out likewise;
+   both 16-byte aligned, the strides multiples of 8 elements and at least
+   n_heads * head_dim; q, out, ws and the cache must not overlap. Query head h
+   reads kv head h / (n_heads / n_kv_heads). ws: a device workspace of
+   attn_workspace_bytes(), 256-byte aligned, that no other call in flight uses
+   (calls on one stream may share it). A wrapped ring takes at most
    capacity - cache sinks - window + 1 queries a call, and no more sinks than
    the cache keeps. Scores, softmax statistics and sums are f32; the weights
    enter the value product rounded to bf16 (with at most 8 query rows per kv

@@ -463,3 +463,45 @@ def test_rope_turns_as_the_models_cache_rows(llama3):
     bound = pair * (p * 2.0 ** -22 + 2.0 ** -20) + (np.abs(got) + np.abs(want)) * 2.0 ** -8
     assert np.all(np.abs(got - want) <= bound)
     assert np.abs(want).max() > 0.01 and not np.array_equal(want[1:], want[:-1])
+
+
+# ------------------------------------------------------------------ two callers at once
+
+def test_attend_on_two_streams_at_once(gen):
+    """Calls of every form on two streams, a workspace each, over one cache and a group of its prefix: the bits of the
+    same calls alone."""
+    c = cache(gen, 4, 128, 3000, 3000)
+    t = cuda.KVGroup(c.kv, 2500, 6, 40)
+    x = rand(gen, 6, 4, 40, 128)
+    for i in range(6):
+        t.write(0, i, 0, x[i].contiguous(), (-x[i]).contiguous())
+    lens = torch.tensor([1, 40, 7, 0, 33, 12], dtype=torch.int32, device="cuda")
+    L, cfg, wide = cuda.lib(), cuda.attn_config(16), cuda.attn_config(32)
+    calls = [(rand(gen, n, h, 128, scale=1.5), pos, a) for n, pos, h, a in ((1, 2999, 16, cfg), (700, 2000, 32, wide),
+                                                                         (40, 2900, 16, cfg), (1, 50, 16, cfg))]
+    qg = rand(gen, 6, 16, 128)
+
+    def passes(ws, st):
+        outs = []
+        for q, pos, a in calls:
+            o = torch.empty_like(q)
+            cuda.check(L.mlxd_cuda_kv_attend(c.kv.kv, 0, q.data_ptr(), q.stride(0), q.shape[0], pos, C.byref(a),
+                                             o.data_ptr(), o.stride(0), ws.data_ptr(), ws.numel(), st), "attend")
+            outs.append(o)
+        o = torch.empty_like(qg)
+        cuda.check(L.mlxd_cuda_kv_group_attend(t.g, 0, qg.data_ptr(), qg.stride(0), lens.data_ptr(), C.byref(cfg),
+                                               o.data_ptr(), o.stride(0), ws.data_ptr(), ws.numel(), st), "group")
+        return outs + [o]
+
+    ws = [torch.empty(cuda.attn_workspace_bytes(128), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    want = passes(ws[0], torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(10):
+        for w, s in zip(ws, streams):
+            with torch.cuda.stream(s):
+                got.append(passes(w, s.cuda_stream))
+    torch.cuda.synchronize()
+    for outs in got:
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
